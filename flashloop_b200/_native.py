@@ -82,6 +82,15 @@ SIGNATURES = {
     "fl_comm_status": (C.c_int, [_vp, C.POINTER(_i32), _i32, _vp]),
     "fl_allreduce_rmsnorm": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _f32, _vp, _f32, _i64, _vp, _vp, _vp, _i32, _i32,
                                        _vp]),
+    "fl_mx_codes_bytes": (_i64, [_i64, _i32, _i32]),
+    "fl_mx_scales_bytes": (_i64, [_i64, _i32]),
+    "fl_mx_quantize": (C.c_int, [_vp, _i32, _i64, _i32, _i64, _i32, _vp, _vp, _vp]),
+    "fl_mx_dequantize": (C.c_int, [_vp, _vp, _i32, _i64, _i32, _vp, _i32, _vp]),
+    "fl_rmsnorm_mx": (C.c_int, [_vp, _vp, _vp, _vp, _f32, _vp, _f32, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "fl_mx_linear": (C.c_int, [_vp, _vp, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _i32, _vp]),
+    "fl_mx_linear_swiglu": (C.c_int, [_vp, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _i32, _i32, _vp,
+                                      _vp]),
+    "fl_mx_status": (C.c_int, [C.POINTER(_i32), _i32, _vp]),
 }
 
 # kernels launched by one call of an entry point (entry points that launch nothing are absent)
@@ -92,6 +101,7 @@ LAUNCHES_PER_CALL = {
     "fl_append_decode_token": 3, "fl_select_decode_keys": 1, "fl_hidden_delta_score": 1,
     "fl_select_prefill_tokens": 1, "fl_gather_rows": 1, "fl_scatter_rows": 1, "fl_encode_prefill": 3, "fl_encode_prefill_stage": 1,
     "fl_rmsnorm": 1, "fl_rope_split": 1, "fl_swiglu": 1, "fl_allreduce_rmsnorm": 1, "fl_linear_rows": 1, "fl_qkv_rope_rows": 1, "fl_linear_rows_partial": 1, "fl_rmsnorm_partial": 1,
+    "fl_mx_quantize": 1, "fl_mx_dequantize": 1, "fl_rmsnorm_mx": 1, "fl_mx_linear": 1, "fl_mx_linear_swiglu": 1,
 }
 
 _LIB = None

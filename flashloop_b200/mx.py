@@ -1,0 +1,277 @@
+"""Microscaled operands: quantisation, the norm that writes them, and the projections that take them
+(``csrc/fl_mx.cu``, ``csrc/fl_mx_linear.cu``).
+
+Thirty-two consecutive elements of a row share a power-of-two scale; the elements are e4m3
+(``"mxfp8"``) or e2m1 (``"mxfp4"``).  The reference's projections are bfloat16
+(flashloop/weights.py:74-117); these are what ``FlashLoopEngine(projection_format=...)`` runs
+instead.  Inference only: no gradient is recorded, and inputs that require one are refused.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _native
+
+FORMATS = {"mxfp8": 0, "mxfp4": 1}
+MAX_NORM_WIDTH = 8192
+
+
+def _format_code(name: str) -> int:
+    try:
+        return FORMATS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"unknown microscaled format {name!r}: use one of {sorted(FORMATS)}") from None
+
+
+def codes_shape(rows: int, cols: int, format: str) -> tuple[int, int]:
+    """Shape of the codes of a [rows, cols] operand."""
+
+    steps = -(-cols // 128)
+    return rows, steps * (128 if _format_code(format) == 0 else 64)
+
+
+def scales_shape(rows: int, cols: int) -> tuple[int, int, int, int, int]:
+    """Shape of its scales: the scale of (row, k) is at [row // 128, k // 128, row % 32, row // 32 % 4, k // 32 % 4]."""
+
+    return -(-rows // 128), -(-cols // 128), 32, 4, 4
+
+
+class MXTensor:
+    """A tensor whose last dimension is held in a microscaled format.
+
+    ``codes`` uint8 (:func:`codes_shape`, elements past the last column zero) and ``scales`` uint8
+    (:func:`scales_shape`, rows past the last zero; byte b stands for 2^(b - 127), 255 for NaN) of
+    ``shape``, whose leading dimensions are the rows.  The tensors are held, not copied."""
+
+    __slots__ = ("codes", "scales", "shape", "format", "rows", "cols", "_code")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, format: str) -> None:
+        shape = tuple(int(v) for v in shape)
+        if not shape or min(shape) < 0 or shape[-1] <= 0:
+            raise ValueError("a microscaled tensor needs at least one dimension and a positive last one")
+        rows = 1
+        for v in shape[:-1]:
+            rows *= v
+        code = _format_code(format)
+        for t, want, name in ((codes, codes_shape(rows, shape[-1], format), "codes"),
+                              (scales, scales_shape(rows, shape[-1]), "scales")):
+            if t.dtype != torch.uint8 or not t.is_contiguous():
+                raise TypeError(f"{name} must be contiguous uint8")
+            if tuple(t.shape) != want:
+                raise ValueError(f"{name} of {shape} in {format} must be {want}, got {tuple(t.shape)}")
+        if codes.device != scales.device:
+            raise ValueError("codes and scales must be on one device")
+        self._set(codes, scales, shape, format, rows, code)
+
+    def _set(self, codes, scales, shape, format, rows, code) -> None:
+        self.codes, self.scales, self.shape, self.format = codes, scales, shape, format
+        self.rows, self.cols, self._code = rows, shape[-1], code
+
+    @classmethod
+    def _empty(cls, shape: tuple, rows: int, format: str, device: torch.device) -> "MXTensor":
+        self = object.__new__(cls)
+        cols, code = shape[-1], _format_code(format)
+        steps = (cols + 127) // 128
+        codes = torch.empty((rows, steps * (64 if code else 128)), dtype=torch.uint8, device=device)
+        scales = torch.empty(((rows + 127) // 128, steps, 32, 4, 4), dtype=torch.uint8, device=device)
+        self._set(codes, scales, shape, format, rows, code)
+        return self
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def __repr__(self) -> str:
+        return f"MXTensor(shape={self.shape}, format={self.format!r}, device={self.codes.device})"
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def view(self, *shape) -> "MXTensor":
+        """The same rows under other leading dimensions."""
+
+        return MXTensor(self.codes, self.scales, shape, self.format)
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The values the codes and scales stand for, rounded to ``dtype``."""
+
+        if dtype not in _native.DTYPE_CODES:
+            raise TypeError("dequantize gives bfloat16, float16 or float32")
+        device = self.codes.device
+        _native.require_cuda(self.codes)
+        out = torch.empty(self.shape, dtype=dtype, device=device)
+        _call(device, "fl_mx_dequantize", self.codes.data_ptr(), self.scales.data_ptr(), self._code, self.rows, self.cols,
+              out.data_ptr(), _native.DTYPE_CODES[dtype])
+        return out
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """One entry point on the current stream of ``device`` (made the current device for the call)."""
+
+    function = getattr(_native.load(), name)
+    if device.index == torch.cuda.current_device():
+        status = function(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            status = function(*args, torch.cuda.current_stream(device).cuda_stream)
+    if status:
+        _native.check(status, name)
+
+
+def _values(*tensors: torch.Tensor | None) -> None:
+    """Floating-point CUDA inputs of one device that need no gradient."""
+
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if t.dtype not in _native.DTYPE_CODES:
+            raise TypeError("microscaled operators take bfloat16, float16 or float32")
+        _native.require_cuda(t)
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise ValueError("all operands must be on one device")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("microscaled operators record no gradient: call them under torch.no_grad()")
+
+
+def mx_quantize(x: torch.Tensor, format: str = "mxfp8") -> MXTensor:
+    """``x`` [..., cols] (bfloat16, float16 or float32; rows of unit inner stride, otherwise copied) in blocks
+    of 32 along the last dimension: the scale is the smallest power of two that keeps the block in
+    range, elements are rounded to nearest, ties to even.  A block with a NaN or an infinity reads
+    as NaN."""
+
+    _values(x)
+    if x.ndim == 0 or x.shape[-1] == 0:
+        raise ValueError("mx_quantize needs at least one column")
+    shape = tuple(x.shape)
+    cols = shape[-1]
+    if x.ndim != 2 or x.stride(1) != 1 or (x.stride(0) < cols and shape[0] > 1):
+        x = x.reshape(-1, cols)  # a view where the rows have one stride
+        if (x.stride(1) != 1 and cols > 1) or (x.stride(0) < cols and x.shape[0] > 1):
+            x = x.contiguous()
+    rows = x.shape[0]
+    q = MXTensor._empty(shape, rows, format, x.device)
+    _call(x.device, "fl_mx_quantize", x.data_ptr(), _native.DTYPE_CODES[x.dtype], rows, cols, x.stride(0), q._code,
+          q.codes.data_ptr(), q.scales.data_ptr())
+    return q
+
+
+def mx_rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: torch.Tensor | None = None,
+               weight2: torch.Tensor | None = None, eps2: float = 0.0, addend: torch.Tensor | None = None,
+               want_sum: bool = False, format: str = "mxfp8"):
+    """RMSNorm with a microscaled result.  ``s = [addend +] x``; without ``weight2`` the result is
+    ``RMSNorm(s)``, with it ``RMSNorm2(hidden)`` of ``hidden = [residual +] RMSNorm(s)``.  ``s`` and
+    ``hidden`` are rounded to the type of ``x``, everything between is float32.  Returns (result
+    :class:`MXTensor`, hidden or None, s or None): s only with ``want_sum``."""
+
+    _values(x, weight, residual, weight2, addend)
+    shape = tuple(x.shape)
+    if not shape or not 0 < shape[-1] <= MAX_NORM_WIDTH:
+        raise ValueError(f"rows must be 1 to {MAX_NORM_WIDTH} wide")
+    width = shape[-1]
+    for t in (weight, weight2):
+        if t is not None and (t.numel() != width or t.dtype != x.dtype or not t.is_contiguous()):
+            raise ValueError("weight does not match the rows")
+    for t in (residual, addend):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError("addend / residual do not match the rows")
+    if residual is not None and weight2 is None:
+        raise ValueError("a residual needs weight2: the stream it is added to is what weight2 normalises")
+    if want_sum and addend is None:
+        raise ValueError("want_sum needs an addend")
+    x = x.contiguous()
+    residual = None if residual is None else residual.contiguous()
+    addend = None if addend is None else addend.contiguous()
+    rows = x.numel() // width
+    q = MXTensor._empty(shape, rows, format, x.device)
+    hidden = None if weight2 is None else torch.empty_like(x)
+    total = torch.empty_like(x) if want_sum else None
+    ptr = _native.ptr
+    _call(x.device, "fl_rmsnorm_mx", x.data_ptr(), ptr(addend), ptr(residual), weight.data_ptr(), eps, ptr(weight2), eps2,
+          _native.DTYPE_CODES[x.dtype], rows, width, q._code, ptr(total), ptr(hidden), q.codes.data_ptr(),
+          q.scales.data_ptr())
+    return q, hidden, total
+
+
+def _operand(x, weight: MXTensor) -> MXTensor:
+    if not isinstance(weight, MXTensor):
+        raise TypeError("the weight must be an MXTensor (mx_quantize)")
+    if len(weight.shape) != 2:
+        raise ValueError("the weight must be [out_features, in_features]")
+    if isinstance(x, torch.Tensor):
+        x = mx_quantize(x, "mxfp8")
+    elif not isinstance(x, MXTensor):
+        raise TypeError("x must be an MXTensor or a tensor to quantise")
+    if x.cols != weight.cols:
+        raise ValueError("x and weight do not match")
+    _native.require_cuda(x.codes, weight.codes)
+    if x.codes.device != weight.codes.device:
+        raise ValueError("all operands must be on one device")
+    return x
+
+
+def mx_linear(x, weight: MXTensor, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``x @ weight.T`` of microscaled operands on the tensor cores, float32 accumulation, rounded once
+    to ``out_dtype``.  ``x`` is an :class:`MXTensor` of either format or a tensor, which is then
+    quantised to mxfp8 first; ``weight`` [out_features, in_features] of either format."""
+
+    x = _operand(x, weight)
+    if out_dtype not in _native.DTYPE_CODES:
+        raise TypeError("out_dtype is bfloat16, float16 or float32")
+    features = weight.shape[0]
+    device = x.codes.device
+    out = torch.empty((*x.shape[:-1], features), dtype=out_dtype, device=device)
+    if out.numel():
+        _call(device, "fl_mx_linear", x.codes.data_ptr(), x.scales.data_ptr(), x._code, weight.codes.data_ptr(),
+              weight.scales.data_ptr(), weight._code, x.rows, features, x.cols, out.data_ptr(),
+              _native.DTYPE_CODES[out_dtype])
+    return out
+
+
+def mx_linear_swiglu(x, gate: MXTensor, up: MXTensor, *, out_dtype: torch.dtype = torch.bfloat16,
+                     out_format: str | None = None):
+    """``silu(x @ gate.T) * (x @ up.T)`` in one launch, as :func:`mx_linear` takes its operands (gate and
+    up of one shape and format).  The activation is float32 and rounded once: to ``out_dtype``, or
+    with ``out_format`` to an :class:`MXTensor`, which the down projection takes as it is."""
+
+    x = _operand(x, gate)
+    _operand(x, up)
+    if gate.shape != up.shape or gate.format != up.format:
+        raise ValueError("gate and up must agree in shape and format")
+    features = gate.shape[0]
+    device = x.codes.device
+    shape = (*x.shape[:-1], features)
+    if out_format is not None:
+        if features == 0:
+            raise ValueError("a microscaled result needs at least one feature")
+        out = MXTensor._empty(shape, x.rows, out_format, device)
+        target, dtype, fmt, scales = out.codes, 0, out._code, out.scales.data_ptr()
+    else:
+        if out_dtype not in _native.DTYPE_CODES:
+            raise TypeError("out_dtype is bfloat16, float16 or float32")
+        out = target = torch.empty(shape, dtype=out_dtype, device=device)
+        dtype, fmt, scales = _native.DTYPE_CODES[out_dtype], 0, None
+    if target.numel():
+        _call(device, "fl_mx_linear_swiglu", x.codes.data_ptr(), x.scales.data_ptr(), x._code, gate.codes.data_ptr(),
+              gate.scales.data_ptr(), up.codes.data_ptr(), up.scales.data_ptr(), gate._code, x.rows, features, x.cols,
+              target.data_ptr(), dtype, fmt, scales)
+    return out
+
+
+def mx_status(device: torch.device | str = "cuda", *, reset: bool = False) -> int:
+    """0, or 1 after a bounded wait inside a microscaled projection ran out on ``device`` (its result was
+    not valid).  Synchronises the current stream."""
+
+    flag = C.c_int32(-1)
+    device = torch.device(device)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    with torch.cuda.device(device):
+        _native.check(_native.load().fl_mx_status(C.byref(flag), int(bool(reset)), _native.current_stream(device)),
+                      "fl_mx_status")
+    return int(flag.value)

@@ -43,6 +43,10 @@ extern "C" {
 #define FL_DTYPE_F16 1
 #define FL_DTYPE_F32 2
 
+/* microscaled formats: 32 elements share a power-of-two scale (e8m0) */
+#define FL_MX_FP8 0 /* e4m3 elements, one byte each */
+#define FL_MX_FP4 1 /* e2m1 elements, two to a byte, the even one in the low nibble */
+
 /* words of fl_layer.seq_state[b] */
 #define FL_STATE_QUANT_TOKENS 0 /* tokens held in the packed streams (multiple of 64)          */
 #define FL_STATE_TAIL_LEN 1     /* tokens held in the BF16 tail                                */
@@ -452,6 +456,66 @@ int fl_rope_split(const void* q_in, const void* k_in, const void* v_in, int64_t 
 /* fused_mlp's activation (flashloop/weights.py:108-117): out = bf16(silu(gate)) * up with
  * gate_up = [rows][2*width] (gate then up), out [rows][width]. */
 int fl_swiglu(const void* gate_up, int64_t rows, int32_t width, void* out, fl_cuda_stream stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Microscaled projections: the decode and prefill projections with both operands in blocks of 32
+ * elements that share a power-of-two scale.  No counterpart in the reference, whose projections
+ * are bfloat16 (flashloop/weights.py:74-117).
+ *
+ * codes  [rows][steps * 128 elements], steps = ceil(cols / 128), elements past cols zero;
+ *        fl_mx_codes_bytes(rows, cols, format) bytes
+ * scales [ceil(rows / 128)][steps][32][4][4] bytes: scale of (row, block k / 32) at
+ *        [row / 128][k / 128][row % 32][row / 32 % 4][k / 32 % 4], byte b standing for 2^(b - 127) and 255 for
+ *        NaN; fl_mx_scales_bytes(rows, cols) bytes, rows past the last holding byte 0
+ * Quantisation: the scale is the smallest power of two (2^-127 or more) that keeps the block within the
+ * format's largest element (448 or 6), elements are rounded to nearest, ties to even.  A block
+ * that holds a NaN or an infinity gets scale 255 and codes 0: all of it reads as NaN.
+ * ------------------------------------------------------------------------------------- */
+
+/* Bytes of the codes and of the scales; 0 for bad sizes.  No counterpart in the reference. */
+int64_t fl_mx_codes_bytes(int64_t rows, int32_t cols, int32_t format);
+/* No counterpart in the reference. */
+int64_t fl_mx_scales_bytes(int64_t rows, int32_t cols);
+
+/* x [rows][cols] of x_dtype, rows row_stride elements apart -> codes and scales (16-byte aligned).
+ * No counterpart in the reference. */
+int fl_mx_quantize(const void* x, int32_t x_dtype, int64_t rows, int32_t cols, int64_t row_stride,
+                   int32_t format, void* codes, void* scales, fl_cuda_stream stream);
+
+/* The values the codes and scales stand for, [rows][cols] of out_dtype.  No counterpart in the reference. */
+int fl_mx_dequantize(const void* codes, const void* scales, int32_t format, int64_t rows, int32_t cols,
+                     void* out, int32_t out_dtype, fl_cuda_stream stream);
+
+/* fl_rmsnorm with a microscaled result (the norm modules of flashloop/engine.py:396, 533-537; the
+ * reference has no such output).  s = x, or with addend s = round(addend + x), stored to sum_out if
+ * given; n = weight * s * rsqrt(mean(s^2) + eps).  Without weight2 the codes are those of n; with it
+ * hidden = round([residual +] n) and the codes are those of weight2 * hidden * rsqrt(mean(hidden^2) +
+ * eps2).  x, addend, residual, weight, weight2, sum_out, hidden are of one dtype, rows contiguous, 1 to
+ * 8192 wide; between the stored tensors everything is float32 (unlike fl_rmsnorm, which rounds where
+ * bfloat16 tensor ops would). */
+int fl_rmsnorm_mx(const void* x, const void* addend, const void* residual, const void* weight, float eps,
+                  const void* weight2, float eps2, int32_t dtype, int64_t rows, int32_t width, int32_t format,
+                  void* sum_out, void* hidden, void* codes, void* scales, fl_cuda_stream stream);
+
+/* out[m][n] = round(sum_k x[m][k] * w[n][k]) over the values the codes and scales of x (rows x
+ * in_features) and w (out_features x in_features) stand for, float32 accumulation; any pairing of
+ * formats; out [rows][out_features] of out_dtype.  Codes 32-byte aligned.  No counterpart in the reference. */
+int fl_mx_linear(const void* x_codes, const void* x_scales, int32_t x_format, const void* w_codes,
+                 const void* w_scales, int32_t w_format, int64_t rows, int32_t out_features,
+                 int32_t in_features, void* out, int32_t out_dtype, fl_cuda_stream stream);
+
+/* silu(x @ gate^T) * (x @ up^T) in float32, rounded to out_dtype, or with out_scales given quantised to
+ * out_format (out then receives the codes).  gate and up have out_features rows each, in one format.
+ * No counterpart in the reference. */
+int fl_mx_linear_swiglu(const void* x_codes, const void* x_scales, int32_t x_format, const void* gate_codes,
+                        const void* gate_scales, const void* up_codes, const void* up_scales,
+                        int32_t w_format, int64_t rows, int32_t out_features, int32_t in_features, void* out,
+                        int32_t out_dtype, int32_t out_format, void* out_scales, fl_cuda_stream stream);
+
+/* *status = 0, or 1 after a bounded wait of fl_mx_linear / fl_mx_linear_swiglu ran out on the current
+ * device since the last reset (that call's result is not valid).  Synchronises `stream`.  No counterpart
+ * in the reference. */
+int fl_mx_status(int32_t* status, int32_t reset, fl_cuda_stream stream);
 
 #ifdef __cplusplus
 }

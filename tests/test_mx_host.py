@@ -1,0 +1,118 @@
+"""Microscaled operators without a GPU: refusals, the container's layout, and the test reference itself."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import flashloop_b200 as fl
+from flashloop_b200 import _native, build_kernels, mx
+from tests import mx_reference as ref
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build_kernels.build()
+    return _native.load()
+
+
+@pytest.mark.parametrize("rows,cols,fmt", [(1, 1, "mxfp8"), (128, 128, "mxfp4"), (129, 129, "mxfp8"), (300, 1000, "mxfp4")])
+def test_shapes_agree_with_the_library(lib, rows, cols, fmt):
+    r, c = mx.codes_shape(rows, cols, fmt)
+    assert r * c == lib.fl_mx_codes_bytes(rows, cols, mx.FORMATS[fmt])
+    assert torch.Size(mx.scales_shape(rows, cols)).numel() == lib.fl_mx_scales_bytes(rows, cols)
+    assert lib.fl_mx_codes_bytes(-1, cols, 0) == lib.fl_mx_codes_bytes(rows, 0, 0) == lib.fl_mx_codes_bytes(rows, cols, 7) == 0
+
+
+def test_reference_quantiser_on_known_blocks():
+    x = torch.zeros(1, 64)
+    x[0, :8] = torch.tensor([6.0, 5.0, 3.5, 2.5, 1.75, 1.25, 0.75, 0.25])  # ties go to the even code
+    x[0, 32] = 6.5  # past the largest element: the next power of two
+    values, byte = ref.quantize(x, "mxfp4")
+    assert values[0, :8].tolist() == [6.0, 4.0, 4.0, 2.0, 2.0, 1.0, 1.0, 0.0]
+    assert byte[0, :2].tolist() == [127, 128] and values[0, 32].item() == 6.0
+    values, byte = ref.quantize(torch.tensor([[448.0] + [float(v) for v in (17, 19, 0.001)]]), "mxfp8")
+    assert byte[0, 0] == 127 and values[0, :3].tolist() == [448.0, 16.0, 20.0]
+    values, byte = ref.quantize(torch.tensor([[1.0, float("inf")]]), "mxfp8")
+    assert byte[0, 0] == 255 and byte[0, 1] == 0 and torch.isnan(values[0, :32]).all()
+
+
+def test_container_checks():
+    codes, scales = torch.zeros(3, 128, dtype=torch.uint8), torch.zeros(1, 1, 32, 4, 4, dtype=torch.uint8)
+    t = fl.MXTensor(codes, scales, (3, 100), "mxfp8")
+    assert (t.rows, t.cols, t.nbytes()) == (3, 100, 3 * 128 + 512)
+    assert t.view(1, 3, 100).shape == (1, 3, 100)
+    with pytest.raises(ValueError):
+        t.view(2, 3, 100)
+    with pytest.raises(ValueError, match="codes"):
+        fl.MXTensor(codes, scales, (3, 100), "mxfp4")
+    with pytest.raises(ValueError, match="scales"):
+        fl.MXTensor(codes, scales[:, :, :16].contiguous(), (3, 100), "mxfp8")
+    with pytest.raises(ValueError, match="unknown microscaled format"):
+        fl.MXTensor(codes, scales, (3, 100), "int4")
+    with pytest.raises(TypeError):
+        fl.MXTensor(codes.int(), scales, (3, 100), "mxfp8")
+    with pytest.raises(TypeError):
+        fl.MXTensor(torch.zeros(128, 3, dtype=torch.uint8).t(), scales, (3, 100), "mxfp8")
+    with pytest.raises(ValueError):
+        fl.MXTensor(codes, scales, (), "mxfp8")
+
+
+def test_refusals_before_the_gpu():
+    x = torch.zeros(2, 64)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        fl.mx_quantize(x)
+    with pytest.raises(TypeError):
+        fl.mx_quantize(x.int())
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        fl.mx_rmsnorm(x, torch.ones(64), 1e-6)
+    with pytest.raises(TypeError):
+        fl.mx_rmsnorm(x.double(), torch.ones(64), 1e-6)
+    weight = fl.MXTensor(torch.zeros(8, 128, dtype=torch.uint8), torch.zeros(1, 1, 32, 4, 4, dtype=torch.uint8), (8, 64), "mxfp8")
+    with pytest.raises(TypeError, match="MXTensor"):
+        fl.mx_linear(weight, x)
+    with pytest.raises(TypeError):
+        fl.mx_linear([1.0], weight)
+    with pytest.raises(ValueError, match="out_features"):
+        fl.mx_linear(weight, weight.view(2, 4, 64))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        fl.mx_linear(weight, weight)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        weight.dequantize()
+    with pytest.raises(TypeError):
+        weight.dequantize(torch.float64)
+
+
+def test_c_refusals(lib):
+    def last():
+        return lib.fl_last_error().decode()
+
+    a = 1 << 20  # an aligned address nothing reads: every call below is refused on the host
+    assert lib.fl_mx_quantize(a, 9, 1, 32, 32, 0, a, a, None) == -1 and "type or format" in last()
+    assert lib.fl_mx_quantize(a, 0, 1, 32, 32, 2, a, a, None) == -1
+    assert lib.fl_mx_quantize(a, 0, 2, 32, 31, 0, a, a, None) == -1 and "bad sizes" in last()
+    assert lib.fl_mx_quantize(None, 0, 1, 32, 32, 0, a, a, None) == -1 and "null" in last()
+    assert lib.fl_mx_quantize(a, 0, 1, 32, 32, 0, a + 8, a, None) == -1 and "aligned" in last()
+    assert lib.fl_mx_quantize(a, 0, 0, 32, 32, 0, None, None, None) == 0
+    assert lib.fl_mx_quantize(a, 0, 1 << 30, 1 << 20, 1 << 20, 0, a, a, None) == -1 and "too many" in last()
+    assert lib.fl_mx_dequantize(a, a, 0, 1, 32, a, 7, None) == -1
+    assert lib.fl_mx_dequantize(a, a, 0, 1, 32, None, 0, None) == -1
+    norm = lambda **k: lib.fl_rmsnorm_mx(*{**dict(x=a, addend=None, residual=None, weight=a, eps=1e-6, weight2=None, eps2=0.0,
+                                                  dtype=0, rows=1, width=64, format=0, sum_out=None, hidden=None, codes=a,
+                                                  scales=a, stream=None), **k}.values())
+    assert norm(width=8193) == -1 and "width" in last()
+    assert norm(width=0) == -1
+    assert norm(weight2=a) == -1 and "go together" in last()
+    assert norm(residual=a) == -1 and "residual" in last()
+    assert norm(sum_out=a) == -1 and "addend" in last()
+    assert norm(x=None) == -1 and norm(codes=a + 4) == -1 and norm(dtype=3) == -1
+    assert norm(rows=0, x=None) == 0
+    assert lib.fl_mx_linear(a, a, 0, a, a, 1, 4, 64, 64, None, 0, None) == -1 and "out" in last()
+    assert lib.fl_mx_linear(a, a, 0, a + 16, a, 1, 4, 64, 64, a, 0, None) == -1 and "32-byte" in last()
+    assert lib.fl_mx_linear(a, a, 5, a, a, 1, 4, 64, 64, a, 0, None) == -1 and "format of x" in last()
+    assert lib.fl_mx_linear(a, a, 0, a, a, 1, 4, 64, 64, a, 3, None) == -1 and "output type" in last()
+    assert lib.fl_mx_linear(a, a, 0, a, a, 1, -1, 64, 64, a, 0, None) == -1
+    assert lib.fl_mx_linear(a, a, 0, a, a, 1, 0, 64, 64, a, 0, None) == 0
+    assert lib.fl_mx_linear_swiglu(a, a, 0, a, a, a, None, 1, 4, 64, 64, a, 0, 0, None, None) == -1 and "null" in last()
+    assert lib.fl_mx_linear_swiglu(a, a, 0, a, a, a, a, 1, 4, 64, 64, a, 0, 4, a, None) == -1 and "output" in last()
+    assert lib.fl_mx_status(None, 0, None) == -1
