@@ -23,7 +23,7 @@ namespace fl {
 namespace {
 
 constexpr int kLinThreads = 192;
-constexpr int kWaitTries = 4096;
+constexpr int kWaitTries = 1 << 15;
 constexpr int kTileW = 128 * 128;  // bytes of a staged weight tile
 constexpr int kMaxStages = 12;
 constexpr int kSmemLimit = 232448;
@@ -57,11 +57,12 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// Acquires at cluster scope: some barriers are arrived at by the other CTAs of a cluster.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
   for (int i = 0; i < kWaitTries; ++i) {
     uint32_t done;
     asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     if (done) return true;
   }
@@ -300,6 +301,273 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   }
 }
 
+// ---------------------------------------------------------------------------------------
+// Many rows of x: persistent CTA pairs (tcgen05 cta_group::2).  A pair computes 256 features by NT
+// rows of x at a time: each CTA stages its 128 features and half of the rows, one thread of the first
+// CTA issues the matrix instructions for both, and each CTA holds [128 features][NT] of the
+// accumulator.  Two accumulators alternate, so the epilogue of one tile runs under the products of
+// the next; beside their 2 * NT columns tensor memory holds the scales of every stage of the ring.
+//
+// silu(gate) * up: the gate tile and the up tile of the same features are two units one after the
+// other; the epilogue moves the gate accumulator to registers while the up products run.
+
+constexpr int kPairThreads = 320;  // copies, matrix instructions, eight epilogue warps
+// NT: rows of x per tile.  A multiple of 64, as the scales of x start at an even column of tensor memory.
+constexpr int kPairRows = 192;
+constexpr int kPairStages = 7;
+constexpr int kPairXTiles = 2;  // scale tiles that 192 rows starting at a multiple of 64 touch
+constexpr int kPairXBytes = kPairRows / 2 * 128;
+constexpr int kPairScalesAt = kTileW + kPairXBytes;
+constexpr int kPairStageBytes = (kPairScalesAt + (1 + kPairXTiles) * kMxTileBytes + 1023) / 1024 * 1024;
+constexpr uint32_t kPairScaleCols = 4 * (1 + kPairXTiles);
+static_assert(kPairXBytes % 1024 == 0, "tiles need 1024-byte alignment");
+static_assert(2 * kPairRows + kPairStages * kPairScaleCols <= 512, "tensor memory columns");
+static_assert(1024 + kPairStages * kPairStageBytes + kTailBytes <= kSmemLimit, "shared memory");
+
+struct PairMaps {
+  CUtensorMap x, x_scales, w[2], w_scales[2];
+};
+
+struct PairParams {
+  void* out;
+  uint8_t* out_scales;
+  int64_t rows;
+  int features;
+  int steps;
+  int w_tiles;       // of 128 features
+  int pair_tiles;    // of 256 features
+  int64_t units;     // tiles times weights
+  uint32_t step_bytes;  // that the copies of one step report, both CTAs
+  uint32_t idesc;
+};
+
+__device__ __forceinline__ void copy_tile_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void scales_to_tmem_pair(uint32_t taddr, uint32_t smem) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(scale_desc(smem)) : "memory");
+}
+__device__ __forceinline__ void mma_mx_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs once every matrix instruction issued so far is done.
+__device__ __forceinline__ void commit_to_both(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+      ::"r"(bar), "h"(uint16_t(3)) : "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+template <int KIND>
+__device__ __forceinline__ void emit_as(const PairParams& p, int64_t m, int n, float v) {
+  if constexpr (KIND <= kOutF32) {
+    if (n >= p.features) return;
+    const int64_t at = m * p.features + n;
+    if constexpr (KIND == kOutBf16) static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+    if constexpr (KIND == kOutF16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
+    if constexpr (KIND == kOutF32) static_cast<float*>(p.out)[at] = v;
+  } else {
+    constexpr int kFormat = KIND == kOutFp8 ? FL_MX_FP8 : FL_MX_FP4;
+    if (n >= p.features) v = 0.f;
+    const uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu);
+    const uint32_t byte = mx_scale_byte<kFormat>(amax);
+    v = byte == 255u ? 0.f : v * mx_inverse(byte);
+    uint8_t* codes = static_cast<uint8_t*>(p.out) + m * (int64_t(p.w_tiles) * (KIND == kOutFp8 ? kMxStep : kMxStep / 2));
+    if constexpr (KIND == kOutFp8) {
+      codes[n] = uint8_t(cvt_e4m3x2(v, 0.f));
+    } else {
+      const float odd = __shfl_down_sync(0xffffffffu, v, 1);
+      if ((n & 1) == 0) codes[n / 2] = uint8_t(cvt_e2m1x2(v, odd));
+    }
+    if ((n & 31) == 0) p.out_scales[mx_scale_offset(m, n / kMxStep, p.w_tiles) + n / kMxBlock % 4] = uint8_t(byte);
+  }
+}
+
+template <int KIND, bool DUAL>
+__global__ void __launch_bounds__(kPairThreads)
+mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* smem = raw_smem + (1024 - (smem_addr(raw_smem) & 1023)) % 1024;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kPairStages * kPairStageBytes);
+  const uint32_t ring = smem_addr(smem), full = smem_addr(bars), empty = full + 8 * kPairStages,
+                 acc_full = empty + 8 * kPairStages, acc_empty = acc_full + 16, drained = acc_empty + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kPairStages + 5);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int64_t pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+  constexpr int kWeights = DUAL ? 2 : 1;
+
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  if (threadIdx.x == 32) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(full + 8 * s, 1);
+      mbar_init(empty + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full + 8 * b, 1);
+      mbar_init(acc_empty + 8 * b, 16);  // a lane of each epilogue warp of both CTAs
+    }
+    mbar_init(drained, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem_scales = tmem + 2 * kPairRows;
+
+  // unit u of this pair: tile t = pair + (u / kWeights) * pairs, weight u % kWeights, features fastest
+  if (warp == 0 && lane == 0) {
+    const uint32_t leader_full = in_cta(full, 0);
+    int64_t issued = 0;
+    bool ok = true;
+    for (int64_t unit = pair * kWeights; ok && unit < p.units;
+         unit += (DUAL && (unit & 1) == 0) ? 1 : pairs * kWeights - (DUAL ? 1 : 0)) {
+      const int64_t tile = unit / kWeights;
+      const int which = int(unit % kWeights);
+      const int w_tile = int(tile % p.pair_tiles) * 2 + int(rank);
+      const int row0 = int(tile / p.pair_tiles) * kPairRows;
+      for (int k = 0; k < p.steps; ++k, ++issued) {
+        const int s = int(issued % kPairStages);
+        if (issued >= kPairStages && !mbar_wait(empty + 8 * s, uint32_t(issued / kPairStages - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        const uint32_t at = ring + s * kPairStageBytes, bar = leader_full + 8 * s;
+        if (rank == 0) mbar_expect(full + 8 * s, p.step_bytes);
+        copy_tile_pair(at, &maps.w[which], k * kMxStep, w_tile * 128, bar);
+        copy_tile_pair(at + kTileW, &maps.x, k * kMxStep, row0 + int(rank) * (kPairRows / 2), bar);
+        copy_tile_pair(at + kPairScalesAt, &maps.w_scales[which], 0, w_tile * p.steps + k, bar);
+#pragma unroll
+        for (int i = 0; i < kPairXTiles; ++i)
+          copy_tile_pair(at + kPairScalesAt + (1 + i) * kMxTileBytes, &maps.x_scales, 0,
+                         (row0 / kMxTileRows + i) * p.steps + k, bar);
+      }
+    }
+    // leave only when every copy of the pair has landed (the last round of the ring)
+    if (rank == 0)
+      for (int64_t i = max(int64_t(0), issued - kPairStages); i < issued; ++i)
+        if (!mbar_wait(full + 8 * int(i % kPairStages), uint32_t(i / kPairStages) & 1)) break;
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    int64_t i = 0;
+    int64_t nth = 0;
+    bool ok = true;
+    for (int64_t unit = pair * kWeights; ok && unit < p.units;
+         unit += (DUAL && (unit & 1) == 0) ? 1 : pairs * kWeights - (DUAL ? 1 : 0), ++nth) {
+      const int buffer = int(nth & 1);
+      const int row0 = int(unit / kWeights / p.pair_tiles) * kPairRows;
+      if (nth >= 2 && !mbar_wait(acc_empty + 8 * buffer, uint32_t(nth / 2 - 1) & 1)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t acc = tmem + buffer * kPairRows;
+      for (int k = 0; k < p.steps; ++k, ++i) {
+        const int s = int(i % kPairStages);
+        if (!mbar_wait(full + 8 * s, uint32_t(i / kPairStages) & 1)) {
+          ok = false;
+          break;
+        }
+        const uint32_t at = ring + s * kPairStageBytes, scales = at + kPairScalesAt;
+        const uint32_t sf = tmem_scales + uint32_t(s) * kPairScaleCols;
+#pragma unroll
+        for (int t = 0; t < 1 + kPairXTiles; ++t) scales_to_tmem_pair(sf + 4 * t, scales + t * kMxTileBytes);
+        const uint64_t w_desc = tile_desc(at), x_desc = tile_desc(at + kTileW);
+        const uint32_t sfb = sf + 4 + (row0 % kMxTileRows) / 32;
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          mma_mx_pair(acc, w_desc + 2 * b, x_desc + 2 * b, p.idesc | uint32_t(b) << 29 | uint32_t(b) << 4, sf, sfb,
+                      k > 0 || b > 0);
+        commit_to_both(empty + 8 * s);
+      }
+      commit_to_both(acc_full + 8 * buffer);
+    }
+    // every product is done before tensor memory is given back
+    commit_to_both(drained);
+    mbar_wait(drained, 0);
+  } else if (warp >= 2) {
+    const uint32_t quarter = uint32_t(warp & 3) * 32, half = uint32_t(warp - 2) / 4;
+    constexpr int kCols = kPairRows / 2;  // this warp's columns of a tile
+    const uint32_t mine = tmem + (quarter << 16) + half * kCols;
+    const uint32_t leader_empty = in_cta(acc_empty, 0);
+    int64_t nth = 0;
+    for (int64_t tile = pair; tile < p.units / kWeights; tile += pairs) {
+      const int n0 = (int(tile % p.pair_tiles) * 2 + int(rank)) * 128;
+      const int n = n0 + int(quarter) + lane;
+      const int64_t m0 = tile / p.pair_tiles * kPairRows + half * kCols;
+      const int cols = n0 < p.features ? int(max(int64_t(0), min(int64_t(kCols), p.rows - m0))) : 0;
+      float gate[DUAL ? kCols : 1];
+      if constexpr (DUAL) {
+        const int buffer = int(nth & 1);
+        if (!mbar_wait(acc_full + 8 * buffer, uint32_t(nth / 2) & 1)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+        for (int c = 0; c < kCols; c += 16) {
+          uint32_t a[16];
+          tmem_load16(mine + buffer * kPairRows + c, a);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int j = 0; j < 16; ++j) gate[c + j] = __uint_as_float(a[j]);
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive_at(leader_empty + 8 * buffer);
+        ++nth;
+      }
+      const int buffer = int(nth & 1);
+      if (!mbar_wait(acc_full + 8 * buffer, uint32_t(nth / 2) & 1)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+      for (int c = 0; c < kCols; c += 16) {
+        uint32_t a[16];
+        tmem_load16(mine + buffer * kPairRows + c, a);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (c + 16 == kCols) {
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) arrive_at(leader_empty + 8 * buffer);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (c + j < cols) {
+            float v = __uint_as_float(a[j]);
+            if constexpr (DUAL) v = gate[c + j] / (1.f + expf(-gate[c + j])) * v;
+            emit_as<KIND>(p, m0 + c + j, n, v);
+          }
+        }
+      }
+      ++nth;
+      // rows of the result's last scale tile past the last row
+      if (KIND > kOutF32 && n0 < p.features && m0 <= p.rows && p.rows <= m0 + kCols) {
+        const int64_t end = (p.rows + kMxTileRows - 1) / kMxTileRows * kMxTileRows;
+        for (int64_t r = p.rows + quarter + lane; r < end; r += 128)
+          *reinterpret_cast<uint32_t*>(p.out_scales + mx_scale_offset(r, n0 / kMxStep, p.w_tiles)) = 0u;
+      }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  }
+  __syncwarp();
+  cluster_sync();
+  if (warp == 0) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
 // ------------------------------------------------------------------------------------ host
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -423,6 +691,85 @@ int launch_linear(const LinearCall& call, int splits) {
   return FL_OK;
 }
 
+// Scale tiles as rows of 128 words; tiles past the last read as zero.
+bool make_scale_map(CUtensorMap* map, const void* scales, int64_t rows, int64_t steps) {
+  const EncodeTiled encode = encode_tiled();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[2] = {kMxTileBytes / 4, cuuint64_t((rows + kMxTileRows - 1) / kMxTileRows * steps)};
+  const cuuint64_t strides[1] = {kMxTileBytes};
+  const cuuint32_t box[2] = {kMxTileBytes / 4, 1};
+  const cuuint32_t unit[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(scales), dims, strides, box, unit,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int KIND, bool DUAL>
+int launch_pairs(const LinearCall& call, int sms) {
+  const int steps = int(mx_steps(call.cols));
+  PairMaps maps;
+  PairParams p;
+  p.out = call.out;
+  p.out_scales = static_cast<uint8_t*>(call.out_scales);
+  p.rows = call.rows;
+  p.features = call.features;
+  p.steps = steps;
+  p.w_tiles = (call.features + 127) / 128;
+  p.pair_tiles = (call.features + 255) / 256;
+  const int64_t tiles = (call.rows + kPairRows - 1) / kPairRows * p.pair_tiles;
+  p.units = tiles * (DUAL ? 2 : 1);
+  p.step_bytes = 2 * uint32_t((kTileW >> (call.w[0].format == FL_MX_FP8 ? 0 : 1)) +
+                              (kPairXBytes >> (call.x.format == FL_MX_FP8 ? 0 : 1)) + (1 + kPairXTiles) * kMxTileBytes);
+  p.idesc = uint32_t(call.w[0].format == FL_MX_FP8 ? 0 : 5) << 7 | uint32_t(call.x.format == FL_MX_FP8 ? 0 : 5) << 10 |
+            uint32_t(kPairRows / 8) << 17 | 1u << 23 | uint32_t(256 / 16) << 24;
+  bool ok = make_map(&maps.x, call.x.codes, call.x.format, call.rows, steps, kPairRows / 2) &&
+            make_scale_map(&maps.x_scales, call.x.scales, call.rows, steps);
+  for (int i = 0; i < 2; ++i) {
+    const Operand& w = call.w[DUAL ? i : 0];
+    ok = ok && make_map(&maps.w[i], w.codes, w.format, call.features, steps, 128) &&
+         make_scale_map(&maps.w_scales[i], w.scales, call.features, steps);
+  }
+  FL_REQUIRE(ok, "%s: the operands cannot be described as tensor maps", call.who);
+  FL_REQUIRE(int64_t(p.w_tiles + 2) * steps < (int64_t(1) << 31) &&
+                 (call.rows / kMxTileRows + kPairXTiles + 1) * steps < (int64_t(1) << 31),
+             "%s: too many elements", call.who);
+  auto kernel = mx_linear_pair_kernel<KIND, DUAL>;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(unsigned(2 * std::min<int64_t>(tiles, sms / 2)));
+  config.blockDim = dim3(kPairThreads);
+  config.dynamicSmemBytes = kSmemLimit;  // all of an SM's, as it takes all of its tensor memory (see above)
+  config.stream = call.stream;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = 2;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  if (err == cudaSuccess) err = cudaLaunchKernelEx(&config, kernel, maps, p);
+  if (err != cudaSuccess) {
+    cudaGetLastError();
+    set_error("%s: %s", call.who, cudaGetErrorString(err));
+    return FL_ERR_CUDA;
+  }
+  return FL_OK;
+}
+
+template <bool DUAL>
+int launch_pairs_of_kind(const LinearCall& call, int sms) {
+  switch (call.out_kind) {
+    case kOutBf16: return launch_pairs<kOutBf16, DUAL>(call, sms);
+    case kOutF16: return launch_pairs<kOutF16, DUAL>(call, sms);
+    case kOutF32: return launch_pairs<kOutF32, DUAL>(call, sms);
+    default: break;
+  }
+  if constexpr (DUAL) {
+    return call.out_kind == kOutFp8 ? launch_pairs<kOutFp8, true>(call, sms) : launch_pairs<kOutFp4, true>(call, sms);
+  } else {
+    FL_REQUIRE(false, "%s: unknown output type", call.who);
+  }
+}
+
 template <bool DUAL>
 int choose_linear(const LinearCall& call) {
   int device = 0;
@@ -439,9 +786,8 @@ int choose_linear(const LinearCall& call) {
   if (call.rows <= 16) return launch_linear<16, DUAL>(call, splits_for(16));
   if (call.rows <= 32) return launch_linear<32, DUAL>(call, splits_for(32));
   if (call.rows <= 64) return launch_linear<64, DUAL>(call, splits_for(64));
-  if constexpr (!DUAL) {
-    if ((call.rows + 255) / 256 * w_tiles >= sms) return launch_linear<256, false>(call, 1);
-  }
+  if ((call.rows + kPairRows - 1) / kPairRows * ((call.features + 255) / 256) >= sms / 2)
+    return launch_pairs_of_kind<DUAL>(call, sms);
   return launch_linear<128, DUAL>(call, splits_for(128));
 }
 
