@@ -57,18 +57,38 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Acquires at cluster scope: some barriers are arrived at by the other CTAs of a cluster.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-  for (int i = 0; i < kWaitTries; ++i) {
-    uint32_t done;
+template <bool CLUSTER>
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  if constexpr (CLUSTER) {  // the barrier is arrived at by the other CTA of a pair
     asm volatile(
         "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-    if (done) return true;
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   }
+  return done != 0;
+}
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+  for (int i = 0; i < kWaitTries; ++i)
+    if (mbar_try<CLUSTER>(bar, parity)) return true;
   atomicExch(&g_mx_status, 1);
   return false;
 }
+// Position in a ring of stages and the parity of its current round.
+struct Ring {
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void advance(int stages) {
+    if (++stage == stages) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+};
 __device__ __forceinline__ void copy_tile(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
@@ -108,6 +128,13 @@ __device__ __forceinline__ void tmem_load16(uint32_t taddr, uint32_t (&r)[16]) {
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
+}
+// One lane of the (converged) warp.  The roles that issue copies and matrix instructions run as whole
+// warps and issue from one lane, so that addresses and descriptors stay in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -174,7 +201,7 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 1);
   const uint32_t ring = smem_addr(smem), full = smem_addr(bars), empty = full + 8 * kMaxStages,
                  done = empty + 8 * kMaxStages;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) / 32, 0), lane = threadIdx.x & 31;
   const uint32_t splits = cluster_size(), rank = cluster_rank();
   const int tile = blockIdx.x / splits;
   const int x_tile = tile / p.w_tiles, w_tile = tile - x_tile * p.w_tiles;
@@ -197,50 +224,58 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const uint32_t tmem_scales = tmem + NT * kWeights;
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     const int x_scale_tiles = int(min(int64_t(kXTiles), (p.rows - row0 + kMxTileRows - 1) / kMxTileRows));
     const uint32_t bytes = p.tile_bytes + (kWeights + x_scale_tiles) * kMxTileBytes;
+    Ring ring_at;
     int issued = 0;
-    for (int k = first; k < last; ++k, ++issued) {
-      const int s = issued % p.stages;
-      if (issued >= p.stages && !mbar_wait(empty + 8 * s, (issued / p.stages - 1) & 1)) break;
+    for (int k = first; k < last; ++k, ++issued, ring_at.advance(p.stages)) {
+      const int s = ring_at.stage;
+      if (issued >= p.stages && !mbar_wait(empty + 8 * s, ring_at.parity ^ 1)) break;
       const uint32_t at = ring + s * kStageBytes, bar = full + 8 * s;
-      mbar_expect(bar, bytes);
-      copy_tile(at, &map_w0, k * kMxStep, w_tile * 128, bar);
-      if (DUAL) copy_tile(at + kTileW, &map_w1, k * kMxStep, w_tile * 128, bar);
-      copy_tile(at + kWeights * kTileW, &map_x, k * kMxStep, int(row0), bar);
-      uint32_t scales = at + kScalesAt;
-      for (int i = 0; i < kWeights; ++i, scales += kMxTileBytes)
-        copy_bytes(scales, p.w_scales[i] + (int64_t(w_tile) * p.steps + k) * kMxTileBytes, kMxTileBytes, bar);
-      for (int i = 0; i < x_scale_tiles; ++i, scales += kMxTileBytes)
-        copy_bytes(scales, p.x_scales + ((row0 / kMxTileRows + i) * p.steps + k) * kMxTileBytes, kMxTileBytes, bar);
+      if (elect_one()) {
+        mbar_expect(bar, bytes);
+        copy_tile(at, &map_w0, k * kMxStep, w_tile * 128, bar);
+        if (DUAL) copy_tile(at + kTileW, &map_w1, k * kMxStep, w_tile * 128, bar);
+        copy_tile(at + kWeights * kTileW, &map_x, k * kMxStep, int(row0), bar);
+        uint32_t scales = at + kScalesAt;
+        for (int i = 0; i < kWeights; ++i, scales += kMxTileBytes)
+          copy_bytes(scales, p.w_scales[i] + (int64_t(w_tile) * p.steps + k) * kMxTileBytes, kMxTileBytes, bar);
+        for (int i = 0; i < x_scale_tiles; ++i, scales += kMxTileBytes)
+          copy_bytes(scales, p.x_scales + ((row0 / kMxTileRows + i) * p.steps + k) * kMxTileBytes, kMxTileBytes, bar);
+      }
+      __syncwarp();
     }
     // leave only when every copy has landed (the last round of the ring)
     for (int i = max(0, issued - p.stages); i < issued; ++i)
-      if (!mbar_wait(full + 8 * (i % p.stages), (i / p.stages) & 1)) break;
-  } else if (warp == 1 && lane == 0) {
-    int i = 0;
-    for (int k = first; k < last; ++k, ++i) {
-      const int s = i % p.stages;
-      if (!mbar_wait(full + 8 * s, (i / p.stages) & 1)) break;
+      if (!mbar_wait(full + 8 * (i % p.stages), uint32_t(i / p.stages) & 1)) break;
+  } else if (warp == 1) {
+    Ring ring_at;
+    for (int k = first; k < last; ++k, ring_at.advance(p.stages)) {
+      const int s = ring_at.stage;
+      if (!mbar_wait(full + 8 * s, ring_at.parity)) break;
       const uint32_t at = ring + s * kStageBytes, scales = at + kScalesAt;
       const uint32_t sf = tmem_scales + s * kScaleCols;
-      for (int t = 0; t < kWeights + kXTiles; ++t) scales_to_tmem(sf + 4 * t, scales + t * kMxTileBytes);
       const uint64_t x_desc = tile_desc(at + kWeights * kTileW);
+      if (elect_one()) {
 #pragma unroll
-      for (int w = 0; w < kWeights; ++w) {
-        const uint64_t w_desc = tile_desc(at + w * kTileW);
+        for (int t = 0; t < kWeights + kXTiles; ++t) scales_to_tmem(sf + 4 * t, scales + t * kMxTileBytes);
 #pragma unroll
-        for (int b = 0; b < 4; ++b)  // a block of 32 elements is 32 bytes along the swizzled row
-          mma_mx(tmem + w * NT, w_desc + 2 * b, x_desc + 2 * b, p.idesc | uint32_t(b) << 29 | uint32_t(b) << 4,
-                 sf + 4 * w, sf + 4 * kWeights, k > first || b > 0);
+        for (int w = 0; w < kWeights; ++w) {
+          const uint64_t w_desc = tile_desc(at + w * kTileW);
+#pragma unroll
+          for (int b = 0; b < 4; ++b)  // a block of 32 elements is 32 bytes along the swizzled row
+            mma_mx(tmem + w * NT, w_desc + 2 * b, x_desc + 2 * b, p.idesc | uint32_t(b) << 29 | uint32_t(b) << 4,
+                   sf + 4 * w, sf + 4 * kWeights, k > first || b > 0);
+        }
+        commit_to(empty + 8 * s);
       }
-      commit_to(empty + 8 * s);
+      __syncwarp();
     }
-    commit_to(done);
+    if (elect_one()) commit_to(done);
   }
   __syncwarp();
 
@@ -405,7 +440,7 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
   const uint32_t ring = smem_addr(smem), full = smem_addr(bars), empty = full + 8 * kPairStages,
                  acc_full = empty + 8 * kPairStages, acc_empty = acc_full + 16, drained = acc_empty + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kPairStages + 5);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) / 32, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int64_t pairs = gridDim.x / 2, pair = blockIdx.x / 2;
   constexpr int kWeights = DUAL ? 2 : 1;
@@ -430,81 +465,95 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   cluster_sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const uint32_t tmem_scales = tmem + 2 * kPairRows;
 
   // unit u of this pair: tile t = pair + (u / kWeights) * pairs, weight u % kWeights, features fastest
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     const uint32_t leader_full = in_cta(full, 0);
-    int64_t issued = 0;
-    bool ok = true;
+    Ring ring_at;
+    bool ok = true, again = false;  // again: the ring has been filled once
     for (int64_t unit = pair * kWeights; ok && unit < p.units;
          unit += (DUAL && (unit & 1) == 0) ? 1 : pairs * kWeights - (DUAL ? 1 : 0)) {
       const int64_t tile = unit / kWeights;
       const int which = int(unit % kWeights);
       const int w_tile = int(tile % p.pair_tiles) * 2 + int(rank);
       const int row0 = int(tile / p.pair_tiles) * kPairRows;
-      for (int k = 0; k < p.steps; ++k, ++issued) {
-        const int s = int(issued % kPairStages);
-        if (issued >= kPairStages && !mbar_wait(empty + 8 * s, uint32_t(issued / kPairStages - 1) & 1)) {
+      for (int k = 0; k < p.steps; ++k) {
+        const int s = ring_at.stage;
+        if (again && !mbar_wait(empty + 8 * s, ring_at.parity ^ 1)) {
           ok = false;
           break;
         }
         const uint32_t at = ring + s * kPairStageBytes, bar = leader_full + 8 * s;
-        if (rank == 0) mbar_expect(full + 8 * s, p.step_bytes);
-        copy_tile_pair(at, &maps.w[which], k * kMxStep, w_tile * 128, bar);
-        copy_tile_pair(at + kTileW, &maps.x, k * kMxStep, row0 + int(rank) * (kPairRows / 2), bar);
-        copy_tile_pair(at + kPairScalesAt, &maps.w_scales[which], 0, w_tile * p.steps + k, bar);
+        if (elect_one()) {
+          if (rank == 0) mbar_expect(full + 8 * s, p.step_bytes);
+          copy_tile_pair(at, &maps.w[which], k * kMxStep, w_tile * 128, bar);
+          copy_tile_pair(at + kTileW, &maps.x, k * kMxStep, row0 + int(rank) * (kPairRows / 2), bar);
+          copy_tile_pair(at + kPairScalesAt, &maps.w_scales[which], 0, w_tile * p.steps + k, bar);
 #pragma unroll
-        for (int i = 0; i < kPairXTiles; ++i)
-          copy_tile_pair(at + kPairScalesAt + (1 + i) * kMxTileBytes, &maps.x_scales, 0,
-                         (row0 / kMxTileRows + i) * p.steps + k, bar);
+          for (int i = 0; i < kPairXTiles; ++i)
+            copy_tile_pair(at + kPairScalesAt + (1 + i) * kMxTileBytes, &maps.x_scales, 0,
+                           (row0 / kMxTileRows + i) * p.steps + k, bar);
+        }
+        __syncwarp();
+        ring_at.advance(kPairStages);
+        again |= ring_at.stage == 0;
       }
     }
-    // leave only when every copy of the pair has landed (the last round of the ring)
-    if (rank == 0)
-      for (int64_t i = max(int64_t(0), issued - kPairStages); i < issued; ++i)
-        if (!mbar_wait(full + 8 * int(i % kPairStages), uint32_t(i / kPairStages) & 1)) break;
-  } else if (warp == 1 && lane == 0 && rank == 0) {
-    int64_t i = 0;
-    int64_t nth = 0;
-    bool ok = true;
+    // leave only when every copy of the pair has landed: the stages of this round, then those of the last
+    if (rank == 0) {
+      for (int s = 0; ok && s < kPairStages; ++s) {
+        const bool this_round = s < ring_at.stage;
+        if (this_round || again) ok = mbar_wait(full + 8 * s, this_round ? ring_at.parity : ring_at.parity ^ 1);
+      }
+    }
+  } else if (warp == 1 && rank == 0) {
+    Ring ring_at, acc_at;
+    bool ok = true, again = false;
     for (int64_t unit = pair * kWeights; ok && unit < p.units;
-         unit += (DUAL && (unit & 1) == 0) ? 1 : pairs * kWeights - (DUAL ? 1 : 0), ++nth) {
-      const int buffer = int(nth & 1);
+         unit += (DUAL && (unit & 1) == 0) ? 1 : pairs * kWeights - (DUAL ? 1 : 0)) {
+      const int buffer = acc_at.stage;
       const int row0 = int(unit / kWeights / p.pair_tiles) * kPairRows;
-      if (nth >= 2 && !mbar_wait(acc_empty + 8 * buffer, uint32_t(nth / 2 - 1) & 1)) break;
+      if (again && !mbar_wait<true>(acc_empty + 8 * buffer, acc_at.parity ^ 1)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t acc = tmem + buffer * kPairRows;
-      for (int k = 0; k < p.steps; ++k, ++i) {
-        const int s = int(i % kPairStages);
-        if (!mbar_wait(full + 8 * s, uint32_t(i / kPairStages) & 1)) {
+      for (int k = 0; k < p.steps; ++k, ring_at.advance(kPairStages)) {
+        const int s = ring_at.stage;
+        if (!mbar_wait(full + 8 * s, ring_at.parity)) {
           ok = false;
           break;
         }
         const uint32_t at = ring + s * kPairStageBytes, scales = at + kPairScalesAt;
         const uint32_t sf = tmem_scales + uint32_t(s) * kPairScaleCols;
-#pragma unroll
-        for (int t = 0; t < 1 + kPairXTiles; ++t) scales_to_tmem_pair(sf + 4 * t, scales + t * kMxTileBytes);
         const uint64_t w_desc = tile_desc(at), x_desc = tile_desc(at + kTileW);
         const uint32_t sfb = sf + 4 + (row0 % kMxTileRows) / 32;
+        if (elect_one()) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-          mma_mx_pair(acc, w_desc + 2 * b, x_desc + 2 * b, p.idesc | uint32_t(b) << 29 | uint32_t(b) << 4, sf, sfb,
-                      k > 0 || b > 0);
-        commit_to_both(empty + 8 * s);
+          for (int t = 0; t < 1 + kPairXTiles; ++t) scales_to_tmem_pair(sf + 4 * t, scales + t * kMxTileBytes);
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            mma_mx_pair(acc, w_desc + 2 * b, x_desc + 2 * b, p.idesc | uint32_t(b) << 29 | uint32_t(b) << 4, sf, sfb,
+                        k > 0 || b > 0);
+          commit_to_both(empty + 8 * s);
+        }
+        __syncwarp();
       }
-      commit_to_both(acc_full + 8 * buffer);
+      if (elect_one()) commit_to_both(acc_full + 8 * buffer);
+      __syncwarp();
+      acc_at.advance(2);
+      again |= acc_at.stage == 0;
     }
     // every product is done before tensor memory is given back
-    commit_to_both(drained);
+    if (elect_one()) commit_to_both(drained);
+    __syncwarp();
     mbar_wait(drained, 0);
   } else if (warp >= 2) {
     const uint32_t quarter = uint32_t(warp & 3) * 32, half = uint32_t(warp - 2) / 4;
     constexpr int kCols = kPairRows / 2;  // this warp's columns of a tile
     const uint32_t mine = tmem + (quarter << 16) + half * kCols;
     const uint32_t leader_empty = in_cta(acc_empty, 0);
-    int64_t nth = 0;
+    Ring acc_at;
     for (int64_t tile = pair; tile < p.units / kWeights; tile += pairs) {
       const int n0 = (int(tile % p.pair_tiles) * 2 + int(rank)) * 128;
       const int n = n0 + int(quarter) + lane;
@@ -512,8 +561,8 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
       const int cols = n0 < p.features ? int(max(int64_t(0), min(int64_t(kCols), p.rows - m0))) : 0;
       float gate[DUAL ? kCols : 1];
       if constexpr (DUAL) {
-        const int buffer = int(nth & 1);
-        if (!mbar_wait(acc_full + 8 * buffer, uint32_t(nth / 2) & 1)) break;
+        const int buffer = acc_at.stage;
+        if (!mbar_wait(acc_full + 8 * buffer, acc_at.parity)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
         for (int c = 0; c < kCols; c += 16) {
@@ -526,10 +575,10 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
         if (lane == 0) arrive_at(leader_empty + 8 * buffer);
-        ++nth;
+        acc_at.advance(2);
       }
-      const int buffer = int(nth & 1);
-      if (!mbar_wait(acc_full + 8 * buffer, uint32_t(nth / 2) & 1)) break;
+      const int buffer = acc_at.stage;
+      if (!mbar_wait(acc_full + 8 * buffer, acc_at.parity)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
       for (int c = 0; c < kCols; c += 16) {
@@ -550,7 +599,7 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
           }
         }
       }
-      ++nth;
+      acc_at.advance(2);
       // rows of the result's last scale tile past the last row
       if (KIND > kOutF32 && n0 < p.features && m0 <= p.rows && p.rows <= m0 + kCols) {
         const int64_t end = (p.rows + kMxTileRows - 1) / kMxTileRows * kMxTileRows;
