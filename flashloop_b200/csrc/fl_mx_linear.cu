@@ -16,6 +16,8 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
+#include <mutex>
 #include <type_traits>
 
 #include "fl_mx_common.cuh"
@@ -27,6 +29,7 @@ constexpr int kLinThreads = 192;
 constexpr int kWaitTries = 1 << 15;
 constexpr int kTileW = 128 * 128;  // bytes of a staged weight tile
 constexpr int kMaxStages = 12;
+constexpr int kMaxSplits = 8;
 constexpr int kSmemLimit = 232448;
 constexpr int kSmemPerSm = 233472;
 constexpr int kTailBytes = 512;  // barriers and the tensor memory base
@@ -34,21 +37,6 @@ constexpr int kTailBytes = 512;  // barriers and the tensor memory base
 __device__ int g_mx_status;
 
 enum OutKind { kOutBf16 = FL_DTYPE_BF16, kOutF16 = FL_DTYPE_F16, kOutF32 = FL_DTYPE_F32, kOutFp8 = 3, kOutFp4 = 4 };
-
-struct LinearParams {
-  const uint8_t *x_scales, *w_scales[2];
-  void* out;            // [rows][features], or the codes of a microscaled result
-  uint8_t* out_scales;  // of a microscaled result
-  int64_t rows;
-  int features;
-  int steps;   // of K
-  int stages;  // of the shared-memory ring
-  int w_tiles;
-  uint32_t tile_bytes;  // that the copies of one step's element tiles report: a spread e2m1 tile counts as packed
-  uint32_t idesc;
-  uint32_t tmem_cols;
-  int out_kind;
-};
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
 
@@ -150,11 +138,18 @@ __device__ __forceinline__ uint32_t cluster_size() {
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ float peer_load(uint32_t addr, uint32_t rank) {
-  float v;
-  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
-               : "=f"(v) : "r"(addr), "r"(rank) : "memory");
-  return v;
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+// Four values into the shared memory of another CTA, counted by its barrier.
+__device__ __forceinline__ void send16(uint32_t cluster_addr, const uint32_t* v, uint32_t cluster_bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+               ::"r"(cluster_addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
 // silu(g) * u.  The exponential and the quotient are the hardware's approximations, a few units in the last place of
@@ -162,183 +157,282 @@ __device__ __forceinline__ float peer_load(uint32_t addr, uint32_t rank) {
 // products take (gated 16384 x 2048 -> 5632: 421 us with expf and a rounded division, 265 us with these and emit16).
 __device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
-// Stores feature n (this thread's) of row m; the 32 lanes of a warp hold 32 consecutive features,
-// which are one block of a microscaled result.  Called by whole warps.
-__device__ __forceinline__ void emit(const LinearParams& p, int64_t m, int n, float v) {
-  if (p.out_kind <= kOutF32) {
-    if (n >= p.features) return;
-    const int64_t at = m * p.features + n;
-    if (p.out_kind == kOutBf16) {
-      static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-    } else if (p.out_kind == kOutF16) {
-      static_cast<__half*>(p.out)[at] = __float2half_rn(v);
-    } else {
-      static_cast<float*>(p.out)[at] = v;
-    }
-    return;
-  }
-  if (n >= p.features) v = 0.f;
-  const uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu);
-  const bool fp8 = p.out_kind == kOutFp8;
-  const uint32_t byte = fp8 ? mx_scale_byte<FL_MX_FP8>(amax) : mx_scale_byte<FL_MX_FP4>(amax);
-  v = byte == 255u ? 0.f : v * mx_inverse(byte);
-  uint8_t* codes = static_cast<uint8_t*>(p.out) + m * (int64_t(p.w_tiles) * (fp8 ? kMxStep : kMxStep / 2));
-  if (fp8) {
-    codes[n] = uint8_t(cvt_e4m3x2(v, 0.f));
+// Where a product goes.
+struct Output {
+  void* data;       // [rows][features], or the codes of a microscaled result
+  uint8_t* scales;  // of a microscaled result
+  int features;
+  int w_tiles;  // of 128 features
+};
+
+// Stores N rows of this thread's feature n, from row m on, of which `count` exist.  The 32 lanes of a
+// warp hold 32 consecutive features, which are one block of a microscaled result; whole warps call it.
+// WHOLE: all N rows and the feature exist.  That path has no branches: the epilogue of many rows is
+// bound by the instructions of its eight warps.
+template <int KIND, bool WHOLE, int N>
+__device__ __forceinline__ void emit_rows(const Output& o, int64_t m, int n, const float (&v)[N], int count) {
+  const bool live = WHOLE || n < o.features;
+  if constexpr (KIND <= kOutF32) {
+    using T = std::conditional_t<KIND == kOutBf16, __nv_bfloat16, std::conditional_t<KIND == kOutF16, __half, float>>;
+    T* dst = static_cast<T*>(o.data) + m * o.features + n;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (WHOLE || (live && j < count)) dst[int64_t(j) * o.features] = round_to<T>(v[j]);
   } else {
-    const float odd = __shfl_down_sync(0xffffffffu, v, 1);
-    if ((n & 1) == 0) codes[n / 2] = uint8_t(cvt_e2m1x2(v, odd));
+    constexpr int kFormat = KIND == kOutFp8 ? FL_MX_FP8 : FL_MX_FP4;
+    const int64_t row_bytes = int64_t(o.w_tiles) * (KIND == kOutFp8 ? kMxStep : kMxStep / 2);
+    uint8_t* codes = static_cast<uint8_t*>(o.data) + m * row_bytes + (KIND == kOutFp8 ? n : n / 2);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (!WHOLE && j >= count) break;  // the same for the warp
+      const float x = live ? v[j] : 0.f;
+      const uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(x) & 0x7fffffffu);
+      const uint32_t byte = mx_scale_byte<kFormat>(amax);
+      const float q = byte == 255u ? 0.f : x * mx_inverse(byte);
+      if constexpr (KIND == kOutFp8) {
+        codes[j * row_bytes] = uint8_t(cvt_e4m3x2(q, 0.f));
+      } else {
+        const float odd = __shfl_down_sync(0xffffffffu, q, 1);
+        if ((n & 1) == 0) codes[j * row_bytes] = uint8_t(cvt_e2m1x2(q, odd));
+      }
+      if ((n & 31) == 0) o.scales[mx_scale_offset(m + j, n / kMxStep, o.w_tiles) + n / kMxBlock % 4] = uint8_t(byte);
+    }
   }
-  if ((n & 31) == 0) p.out_scales[mx_scale_offset(m, n / kMxStep, p.w_tiles) + n / kMxBlock % 4] = uint8_t(byte);
+}
+// The scales of the result's last tile past its last row, for 128 features from n0 on: zero.
+__device__ __forceinline__ void zero_scales(const Output& o, int64_t rows, int n0, int thread, int threads) {
+  const int64_t end = (rows + kMxTileRows - 1) / kMxTileRows * kMxTileRows;
+  for (int64_t r = rows + thread; r < end; r += threads)
+    *reinterpret_cast<uint32_t*>(o.scales + mx_scale_offset(r, n0 / kMxStep, o.w_tiles)) = 0u;
 }
 
+struct LinearParams {
+  const uint8_t *x_scales, *w_scales[2];
+  Output out;
+  int64_t rows;
+  int steps;   // of K
+  int stages;  // of the shared-memory ring
+  uint32_t w_bytes, x_bytes;  // that the copies of one step's tiles report: a spread e2m1 tile counts as packed
+  uint32_t idesc;
+  uint32_t tmem_cols;
+};
+
+// Shared memory of the kernel for few rows.
 template <int NT, bool DUAL>
+struct FewRows {
+  static constexpr int kWeights = DUAL ? 2 : 1;
+  static constexpr int kXBytes = NT * 128;
+  static constexpr int kScalesAt = kWeights * kTileW + kXBytes;
+  static constexpr int kStageBytes = (kScalesAt + (kWeights + 1) * kMxTileBytes + 1023) / 1024 * 1024;
+  static constexpr uint32_t kScaleCols = 4 * (kWeights + 1);  // tensor memory columns of a stage's scales
+  // groups of four columns of the accumulator that a CTA of a split finishes, and the shared memory in which
+  // it receives them from every CTA of its cluster: [source][weight][group][feature][column of the group]
+  static constexpr __host__ __device__ int groups(int splits, int cols) {
+    return ((cols + 3) / 4 + splits - 1) / splits;
+  }
+  static int exchange_bytes(int splits, int cols) {
+    return splits > 1 ? splits * kWeights * groups(splits, cols) * 2048 : 0;
+  }
+};
+
+// Few rows of x: a CTA computes 128 features by NT rows over its share of K.  What such a call
+// takes is latency, so the copies start before anything else, issued by four warps, and a split sends
+// its sums straight into the shared memory of the CTA that finishes them, which waits for their bytes.
+template <int KIND, int NT, bool DUAL>
 __global__ void __launch_bounds__(kLinThreads)
 mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w0,
                  const __grid_constant__ CUtensorMap map_w1, const LinearParams p) {
-  constexpr int kWeights = DUAL ? 2 : 1;
-  constexpr int kXTiles = NT > 128 ? NT / 128 : 1;  // scale tiles of the x rows of a step
-  constexpr int kScalesAt = kWeights * kTileW + NT * 128;
-  constexpr int kStageBytes = (kScalesAt + (kWeights + kXTiles) * kMxTileBytes + 1023) / 1024 * 1024;
-  constexpr uint32_t kScaleCols = 4 * (kWeights + kXTiles);  // tensor memory columns of a stage's scales
+  using Shape = FewRows<NT, DUAL>;
+  constexpr int kWeights = Shape::kWeights, kStageBytes = Shape::kStageBytes, kScalesAt = Shape::kScalesAt;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* smem = raw_smem + (1024 - (smem_addr(raw_smem) & 1023)) % 1024;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + p.stages * kStageBytes);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 2);
+  float4* exchange = reinterpret_cast<float4*>(smem + p.stages * kStageBytes + kTailBytes);
   const uint32_t ring = smem_addr(smem), full = smem_addr(bars), empty = full + 8 * kMaxStages,
-                 done = empty + 8 * kMaxStages;
+                 done = empty + 8 * kMaxStages, received = done + 8;
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) / 32, 0), lane = threadIdx.x & 31;
-  const uint32_t splits = cluster_size(), rank = cluster_rank();
+  const int splits = int(cluster_size()), rank = int(cluster_rank());
   const int tile = blockIdx.x / splits;
-  const int x_tile = tile / p.w_tiles, w_tile = tile - x_tile * p.w_tiles;
-  const int64_t row0 = int64_t(x_tile) * NT;
-  const int first = int(int64_t(p.steps) * rank / splits), last = int(int64_t(p.steps) * (rank + 1) / splits);
+  const int x_tile = tile / p.out.w_tiles, w_tile = tile - x_tile * p.out.w_tiles;
+  const int row0 = x_tile * NT;  // NT < 128 only where there is one tile of x or NT divides 128
+  const int first = p.steps * rank / splits, last = p.steps * (rank + 1) / splits;
+
+  const int cols = int(min(int64_t(NT), p.rows - row0));
+  const int groups = Shape::groups(splits, cols);  // that each CTA of a split finishes
+  const int my_groups = max(0, min(groups, (cols + 3) / 4 - rank * groups));
 
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
-                 "r"(p.tmem_cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  if (threadIdx.x == 32) {
-    for (int s = 0; s < p.stages; ++s) {
-      mbar_init(full + 8 * s, 1);
-      mbar_init(empty + 8 * s, 1);
+    if (lane < p.stages) {
+      mbar_init(full + 8 * lane, 4);  // the four warps that copy
+      mbar_init(empty + 8 * lane, 1);
+    } else if (lane == 30) {
+      mbar_init(done, 1);
+    } else if (lane == 31) {
+      mbar_init(received, 1);
+      if (splits > 1) mbar_expect(received, uint32_t(splits * kWeights * my_groups) * 2048);
     }
-    mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-  const uint32_t tmem_scales = tmem + NT * kWeights;
-
-  if (warp == 0) {
-    const int x_scale_tiles = int(min(int64_t(kXTiles), (p.rows - row0 + kMxTileRows - 1) / kMxTileRows));
-    const uint32_t bytes = p.tile_bytes + (kWeights + x_scale_tiles) * kMxTileBytes;
-    Ring ring_at;
-    int issued = 0;
-    for (int k = first; k < last; ++k, ++issued, ring_at.advance(p.stages)) {
-      const int s = ring_at.stage;
-      if (issued >= p.stages && !mbar_wait(empty + 8 * s, ring_at.parity ^ 1)) break;
-      const uint32_t at = ring + s * kStageBytes, bar = full + 8 * s;
-      if (elect_one()) {
-        mbar_expect(bar, bytes);
-        copy_tile(at, &map_w0, k * kMxStep, w_tile * 128, bar);
-        if (DUAL) copy_tile(at + kTileW, &map_w1, k * kMxStep, w_tile * 128, bar);
-        copy_tile(at + kWeights * kTileW, &map_x, k * kMxStep, int(row0), bar);
-        uint32_t scales = at + kScalesAt;
-        for (int i = 0; i < kWeights; ++i, scales += kMxTileBytes)
-          copy_bytes(scales, p.w_scales[i] + (int64_t(w_tile) * p.steps + k) * kMxTileBytes, kMxTileBytes, bar);
-        for (int i = 0; i < x_scale_tiles; ++i, scales += kMxTileBytes)
-          copy_bytes(scales, p.x_scales + ((row0 / kMxTileRows + i) * p.steps + k) * kMxTileBytes, kMxTileBytes, bar);
-      }
-      __syncwarp();
-    }
-    // leave only when every copy has landed (the last round of the ring)
-    for (int i = max(0, issued - p.stages); i < issued; ++i)
-      if (!mbar_wait(full + 8 * (i % p.stages), uint32_t(i / p.stages) & 1)) break;
   } else if (warp == 1) {
+    if (lane == 0) {
+      prefetch_map(&map_w0);
+      prefetch_map(&map_x);
+      if (DUAL) prefetch_map(&map_w1);
+    }
+  }
+  __syncthreads();
+  if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA runs
+
+  if (warp == 0 || (warp >= 2 && warp <= 4)) {
+    // warp 0: weight tiles; 2: rows of x; 3: scales of x; 4: scales of the weights
+    const uint8_t* x_scales = p.x_scales + int64_t(row0 / kMxTileRows) * p.steps * kMxTileBytes;
+    const int64_t w_scales_at = int64_t(w_tile) * p.steps * kMxTileBytes;
     Ring ring_at;
     for (int k = first; k < last; ++k, ring_at.advance(p.stages)) {
       const int s = ring_at.stage;
-      if (!mbar_wait(full + 8 * s, ring_at.parity)) break;
+      if (k - first >= p.stages && !mbar_wait(empty + 8 * s, ring_at.parity ^ 1)) break;
+      const uint32_t at = ring + s * kStageBytes, bar = full + 8 * s;
+      if (elect_one()) {
+        if (warp == 0) {
+          mbar_expect(bar, kWeights * p.w_bytes);
+          copy_tile(at, &map_w0, k * kMxStep, w_tile * 128, bar);
+          if (DUAL) copy_tile(at + kTileW, &map_w1, k * kMxStep, w_tile * 128, bar);
+        } else if (warp == 2) {
+          mbar_expect(bar, p.x_bytes);
+          copy_tile(at + kWeights * kTileW, &map_x, k * kMxStep, row0, bar);
+        } else if (warp == 3) {
+          mbar_expect(bar, kMxTileBytes);
+          copy_bytes(at + kScalesAt + kWeights * kMxTileBytes, x_scales + int64_t(k) * kMxTileBytes, kMxTileBytes, bar);
+        } else {
+          mbar_expect(bar, kWeights * kMxTileBytes);
+          for (int i = 0; i < kWeights; ++i)
+            copy_bytes(at + kScalesAt + i * kMxTileBytes, p.w_scales[i] + w_scales_at + int64_t(k) * kMxTileBytes,
+                       kMxTileBytes, bar);
+        }
+      }
+      __syncwarp();
+    }
+  } else if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                 "r"(p.tmem_cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    __syncwarp();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    asm volatile("bar.arrive 1, 160;" ::: "memory");  // the epilogue may read the slot
+    const uint32_t tmem_scales = tmem + NT * kWeights;
+    // scales of x: NT rows of a 128-row tile start at its column (row0 % 128) / 32, an even one
+    const uint32_t x_col = 4 * kWeights + uint32_t(row0 % kMxTileRows) / 32;
+    Ring ring_at;
+    bool ok = true;
+    for (int k = first; k < last; ++k, ring_at.advance(p.stages)) {
+      const int s = ring_at.stage;
+      ok = mbar_wait(full + 8 * s, ring_at.parity);
+      if (!ok) break;
       const uint32_t at = ring + s * kStageBytes, scales = at + kScalesAt;
-      const uint32_t sf = tmem_scales + s * kScaleCols;
+      const uint32_t sf = tmem_scales + s * Shape::kScaleCols;
       const uint64_t x_desc = tile_desc(at + kWeights * kTileW);
       if (elect_one()) {
 #pragma unroll
-        for (int t = 0; t < kWeights + kXTiles; ++t) scales_to_tmem(sf + 4 * t, scales + t * kMxTileBytes);
+        for (int t = 0; t < kWeights + 1; ++t) scales_to_tmem(sf + 4 * t, scales + t * kMxTileBytes);
 #pragma unroll
         for (int w = 0; w < kWeights; ++w) {
           const uint64_t w_desc = tile_desc(at + w * kTileW);
 #pragma unroll
           for (int b = 0; b < 4; ++b)  // a block of 32 elements is 32 bytes along the swizzled row
             mma_mx(tmem + w * NT, w_desc + 2 * b, x_desc + 2 * b, p.idesc | uint32_t(b) << 29 | uint32_t(b) << 4,
-                   sf + 4 * w, sf + 4 * kWeights, k > first || b > 0);
+                   sf + 4 * w, sf + x_col, k > first || b > 0);
         }
         commit_to(empty + 8 * s);
       }
       __syncwarp();
     }
     if (elect_one()) commit_to(done);
+    __syncwarp();
+    // after a wait that ran out: copies may still be landing
+    if (!ok)
+      for (int s = 0; s < p.stages; ++s) mbar_wait(full + 8 * s, ring_at.parity);
   }
   __syncwarp();
 
   const int n = w_tile * 128 + (warp & 3) * 32 + lane;
-  const int cols = int(min(int64_t(NT), p.rows - row0));
+  const bool features_whole = w_tile * 128 + 128 <= p.out.features;
   if (warp >= 2) {
+    asm volatile("bar.sync 1, 160;" ::: "memory");
+    const uint32_t acc = __shfl_sync(0xffffffffu, *tmem_slot, 0) + (uint32_t(warp & 3) * 32 << 16);
     mbar_wait(done, 0);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t mine = tmem + (uint32_t(warp & 3) * 32 << 16);
-    float* partial = reinterpret_cast<float*>(smem) + (warp & 3) * 32 + lane;  // [weight][column][feature]
-    for (int c = 0; c < cols; c += 16) {
-      uint32_t a[16], b[16];
-      tmem_load16(mine + c, a);
-      if (DUAL) tmem_load16(mine + NT + c, b);
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    if (splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all of the cluster run
+    const int feature = (warp & 3) * 32 + lane;
+    const uint32_t slot = smem_addr(exchange) + uint32_t(rank * kWeights * groups * 128 + feature) * 16;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (c + j >= cols) break;
-        float v = __uint_as_float(a[j]);
-        if (splits > 1) {
-          partial[(c + j) * 128] = v;
-          if (DUAL) partial[(NT + c + j) * 128] = __uint_as_float(b[j]);
+    for (int c = 0; c < NT; c += 16) {
+      if (c >= cols) break;
+      uint32_t a[16], b[16];
+      tmem_load16(acc + c, a);
+      if (DUAL) tmem_load16(acc + NT + c, b);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      if (splits > 1) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          if (c + j < cols) {
+            const int group = (c + j) / 4, owner = group / groups, at = group - owner * groups;
+            const uint32_t bar = in_cta(received, uint32_t(owner));
+            const uint32_t dst = in_cta(slot + uint32_t(at) * 2048, uint32_t(owner));
+            send16(dst, a + j, bar);
+            if (DUAL) send16(dst + uint32_t(groups) * 2048, b + j, bar);
+          }
+        }
+      } else {
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          v[j] = DUAL ? gated(__uint_as_float(a[j]), __uint_as_float(b[j])) : __uint_as_float(a[j]);
+        if (features_whole && c + 16 <= cols) {
+          emit_rows<KIND, true>(p.out, row0 + c, n, v, 16);
         } else {
-          if (DUAL) v = gated(v, __uint_as_float(b[j]));
-          emit(p, row0 + c + j, n, v);
+          emit_rows<KIND, false>(p.out, row0 + c, n, v, cols - c);
         }
       }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  }
-  if (splits > 1) {
-    cluster_sync();
-    if (warp >= 2) {
-      const uint32_t mine = ring + ((warp & 3) * 32 + lane) * 4;
-      for (int c = rank; c < cols; c += splits) {
-        float v = 0.f, u = 0.f;
-        for (uint32_t r = 0; r < splits; ++r) {
-          v += peer_load(mine + c * 512, r);
-          if (DUAL) u += peer_load(mine + (NT + c) * 512, r);
+    if (splits > 1 && my_groups > 0) {
+      // The other CTAs always send, also after a wait of theirs has run out: wait as long as they may take.
+      for (int i = 0; i < 16 && !mbar_wait<true>(received, 0); ++i) {
+      }
+      for (int g = 0; g < my_groups; ++g) {
+        const float4* src = exchange + g * 128 + feature;
+        float v[4] = {}, u[4] = {};
+#pragma unroll
+        for (int r = 0; r < kMaxSplits; ++r) {  // in rank order
+          if (r < splits) {
+            const float4 t = src[r * kWeights * groups * 128];
+            v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
+            if (DUAL) {
+              const float4 w = src[(r * kWeights + 1) * groups * 128];
+              u[0] += w.x; u[1] += w.y; u[2] += w.z; u[3] += w.w;
+            }
+          }
         }
-        if (DUAL) v = gated(v, u);
-        emit(p, row0 + c, n, v);
+        if (DUAL) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = gated(v[j], u[j]);
+        }
+        const int c = (rank * groups + g) * 4;
+        if (features_whole && c + 4 <= cols) {
+          emit_rows<KIND, true>(p.out, row0 + c, n, v, 4);
+        } else {
+          emit_rows<KIND, false>(p.out, row0 + c, n, v, cols - c);
+        }
       }
     }
-    cluster_sync();
-  } else {
-    __syncthreads();
+  } else if (splits > 1) {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
-  // rows of the result's last scale tile past the last row
-  if (p.out_kind > kOutF32 && rank == 0 && row0 + NT >= p.rows) {
-    const int64_t end = (p.rows + kMxTileRows - 1) / kMxTileRows * kMxTileRows;
-    for (int64_t r = p.rows + threadIdx.x; r < end; r += kLinThreads)
-      *reinterpret_cast<uint32_t*>(p.out_scales + mx_scale_offset(r, w_tile, p.w_tiles)) = 0u;
-  }
-  if (warp == 0) {
+  if (KIND > kOutF32 && rank == 0 && row0 + NT >= p.rows) zero_scales(p.out, p.rows, w_tile * 128, threadIdx.x, kLinThreads);
+  __syncthreads();
+  if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(p.tmem_cols) : "memory");
   }
 }
 
@@ -370,12 +464,9 @@ struct PairMaps {
 };
 
 struct PairParams {
-  void* out;
-  uint8_t* out_scales;
+  Output out;
   int64_t rows;
-  int features;
   int steps;
-  int w_tiles;       // of 128 features
   int pair_tiles;    // of 256 features
   int64_t units;     // tiles times weights
   uint32_t step_bytes;  // that the copies of one step report, both CTAs
@@ -403,48 +494,8 @@ __device__ __forceinline__ void commit_to_both(uint32_t bar) {
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
       ::"r"(bar), "h"(uint16_t(3)) : "memory");
 }
-__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
-  uint32_t a;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  return a;
-}
 __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
-}
-
-// Stores sixteen rows of this thread's feature n, from row m on, of which `count` exist; whole warps call
-// it.  WHOLE: all sixteen, and the feature exists.  That path has no branches: the epilogue is bound by
-// the instructions of its eight warps.
-template <int KIND, bool WHOLE>
-__device__ __forceinline__ void emit16(const PairParams& p, int64_t m, int n, const float (&v)[16], int count) {
-  const bool live = WHOLE || n < p.features;
-  if constexpr (KIND <= kOutF32) {
-    using T = std::conditional_t<KIND == kOutBf16, __nv_bfloat16, std::conditional_t<KIND == kOutF16, __half, float>>;
-    T* dst = static_cast<T*>(p.out) + m * p.features + n;
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (WHOLE || (live && j < count)) dst[int64_t(j) * p.features] = round_to<T>(v[j]);
-  } else {
-    constexpr int kFormat = KIND == kOutFp8 ? FL_MX_FP8 : FL_MX_FP4;
-    const int64_t row_bytes = int64_t(p.w_tiles) * (KIND == kOutFp8 ? kMxStep : kMxStep / 2);
-    uint8_t* codes = static_cast<uint8_t*>(p.out) + m * row_bytes + (KIND == kOutFp8 ? n : n / 2);
-    uint8_t* scale = p.out_scales + mx_scale_offset(m, n / kMxStep, p.w_tiles) + n / kMxBlock % 4;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      if (!WHOLE && j >= count) break;  // the same for the warp
-      const float x = live ? v[j] : 0.f;
-      const uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(x) & 0x7fffffffu);
-      const uint32_t byte = mx_scale_byte<kFormat>(amax);
-      const float q = byte == 255u ? 0.f : x * mx_inverse(byte);
-      if constexpr (KIND == kOutFp8) {
-        codes[j * row_bytes] = uint8_t(cvt_e4m3x2(q, 0.f));
-      } else {
-        const float odd = __shfl_down_sync(0xffffffffu, q, 1);
-        if ((n & 1) == 0) codes[j * row_bytes] = uint8_t(cvt_e2m1x2(q, odd));
-      }
-      if ((n & 31) == 0) scale[j * 16] = uint8_t(byte);  // sixteen rows from a multiple of 16 on share a lane group
-    }
-  }
 }
 
 template <int KIND, bool DUAL>
@@ -574,8 +625,8 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
       const int n0 = (int(tile % p.pair_tiles) * 2 + int(rank)) * 128;
       const int n = n0 + int(quarter) + lane;
       const int64_t m0 = tile / p.pair_tiles * kPairRows + half * kCols;
-      const int cols = n0 < p.features ? int(max(int64_t(0), min(int64_t(kCols), p.rows - m0))) : 0;
-      const bool whole = cols == kCols && n0 + 128 <= p.features;
+      const int cols = n0 < p.out.features ? int(max(int64_t(0), min(int64_t(kCols), p.rows - m0))) : 0;
+      const bool whole = cols == kCols && n0 + 128 <= p.out.features;
       float gate[DUAL ? kCols : 1];
       if constexpr (DUAL) {
         const int buffer = acc_at.stage;
@@ -611,18 +662,14 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = DUAL ? gated(gate[DUAL ? c + j : 0], __uint_as_float(a[j])) : __uint_as_float(a[j]);
         if (whole) {
-          emit16<KIND, true>(p, m0 + c, n, v, 16);
+          emit_rows<KIND, true>(p.out, m0 + c, n, v, 16);
         } else if (c < cols) {
-          emit16<KIND, false>(p, m0 + c, n, v, cols - c);
+          emit_rows<KIND, false>(p.out, m0 + c, n, v, cols - c);
         }
       }
       acc_at.advance(2);
-      // rows of the result's last scale tile past the last row
-      if (KIND > kOutF32 && n0 < p.features && m0 <= p.rows && p.rows <= m0 + kCols) {
-        const int64_t end = (p.rows + kMxTileRows - 1) / kMxTileRows * kMxTileRows;
-        for (int64_t r = p.rows + quarter + lane; r < end; r += 128)
-          *reinterpret_cast<uint32_t*>(p.out_scales + mx_scale_offset(r, n0 / kMxStep, p.w_tiles)) = 0u;
-      }
+      if (KIND > kOutF32 && n0 < p.out.features && m0 <= p.rows && p.rows <= m0 + kCols)
+        zero_scales(p.out, p.rows, n0, int(quarter) + lane, 128);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
@@ -670,15 +717,13 @@ bool make_map(CUtensorMap* map, const void* codes, int format, int64_t rows, int
 
 constexpr int kMaxDevices = 64;
 
-int sm_count(int device) {
-  static int counts[kMaxDevices];  // written with the same value by whoever comes first
-  if (device < 0 || device >= kMaxDevices) return 148;
-  if (counts[device] == 0) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) n = 148;
-    counts[device] = n;
-  }
-  return counts[device];
+// Lets a kernel use all of an SM's shared memory, once per device.
+template <typename K>
+cudaError_t allow_shared_memory(K kernel, std::atomic<bool> (&done)[kMaxDevices], int device) {
+  if (done[device].load(std::memory_order_acquire)) return cudaSuccess;
+  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+  if (err == cudaSuccess) done[device].store(true, std::memory_order_release);
+  return err;
 }
 
 struct Operand {
@@ -694,49 +739,48 @@ struct LinearCall {
   void *out, *out_scales;
   cudaStream_t stream;
   const char* who;
+  int device;
 };
 
-template <int NT, bool DUAL>
-int launch_linear(const LinearCall& call, int splits) {
-  constexpr int kWeights = DUAL ? 2 : 1, kXTiles = NT > 128 ? NT / 128 : 1;
-  constexpr int kStageBytes =
-      (kWeights * kTileW + NT * 128 + (kWeights + kXTiles) * kMxTileBytes + 1023) / 1024 * 1024;
-  constexpr int kScaleCols = 4 * (kWeights + kXTiles);
-  constexpr int kPartialBytes = kWeights * NT * 512;
+template <int KIND, int NT, bool DUAL>
+int launch_linear(const LinearCall& call, int splits, int most_stages) {
+  using Shape = FewRows<NT, DUAL>;
   const int steps = int(mx_steps(call.cols));
   LinearParams p;
   p.x_scales = static_cast<const uint8_t*>(call.x.scales);
   p.w_scales[0] = static_cast<const uint8_t*>(call.w[0].scales);
   p.w_scales[1] = static_cast<const uint8_t*>(call.w[1].scales);
-  p.out = call.out;
-  p.out_scales = static_cast<uint8_t*>(call.out_scales);
+  p.out = Output{call.out, static_cast<uint8_t*>(call.out_scales), call.features, (call.features + 127) / 128};
   p.rows = call.rows;
-  p.features = call.features;
   p.steps = steps;
-  p.w_tiles = (call.features + 127) / 128;
-  p.out_kind = call.out_kind;
-  p.tile_bytes = uint32_t((kWeights * kTileW >> (call.w[0].format == FL_MX_FP8 ? 0 : 1)) +
-                          (NT * 128 >> (call.x.format == FL_MX_FP8 ? 0 : 1)));
-  const int most = std::min(kMaxStages, (kSmemLimit - 1024 - kTailBytes) / kStageBytes);
-  p.stages = std::min(most, (steps + splits - 1) / splits);
-  const int need = NT * kWeights + p.stages * kScaleCols;
+  p.w_bytes = uint32_t(kTileW >> (call.w[0].format == FL_MX_FP8 ? 0 : 1));
+  p.x_bytes = uint32_t(Shape::kXBytes >> (call.x.format == FL_MX_FP8 ? 0 : 1));
+  const int exchange = Shape::exchange_bytes(splits, int(std::min<int64_t>(NT, call.rows)));
+  const int room = (kSmemLimit - 1024 - kTailBytes - exchange) / Shape::kStageBytes;
+  p.stages = std::min({kMaxStages, room, most_stages, (steps + splits - 1) / splits});
+  const int need = NT * Shape::kWeights + p.stages * int(Shape::kScaleCols);
   p.tmem_cols = need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
   // Shared memory in proportion to the columns: CTAs of these kernels that fit an SM together
   // never want more than its 512 columns, so none waits for columns while its cluster waits for it.
-  const int smem = std::max({1024 + kTailBytes + std::max(p.stages * kStageBytes, splits > 1 ? kPartialBytes : 0),
-                             int(p.tmem_cols) * (kSmemPerSm / 512) - 1024});
+  const int smem = std::max(1024 + kTailBytes + p.stages * Shape::kStageBytes + exchange,
+                            int(p.tmem_cols) * (kSmemPerSm / 512) - 1024);
   // instruction descriptor: element types (e4m3 0, e2m1 5), e8m0 scales, N, M = 128
   p.idesc = uint32_t(call.w[0].format == FL_MX_FP8 ? 0 : 5) << 7 | uint32_t(call.x.format == FL_MX_FP8 ? 0 : 5) << 10 |
             uint32_t(NT / 8) << 17 | 1u << 23 | uint32_t(128 / 16) << 24;
   CUtensorMap map_x, map_w0, map_w1;
-  FL_REQUIRE(make_map(&map_x, call.x.codes, call.x.format, call.rows, steps, NT) &&
-                 make_map(&map_w0, call.w[0].codes, call.w[0].format, call.features, steps, 128) &&
-                 make_map(&map_w1, call.w[DUAL ? 1 : 0].codes, call.w[0].format, call.features, steps, 128),
-             "%s: the operands cannot be described as tensor maps", call.who);
-  const int64_t tiles = (call.rows + NT - 1) / NT * p.w_tiles;
+  bool ok = make_map(&map_x, call.x.codes, call.x.format, call.rows, steps, NT) &&
+            make_map(&map_w0, call.w[0].codes, call.w[0].format, call.features, steps, 128);
+  if (DUAL) {
+    ok = ok && make_map(&map_w1, call.w[1].codes, call.w[1].format, call.features, steps, 128);
+  } else {
+    map_w1 = map_w0;
+  }
+  FL_REQUIRE(ok, "%s: the operands cannot be described as tensor maps", call.who);
+  const int64_t tiles = (call.rows + NT - 1) / NT * p.out.w_tiles;
   FL_REQUIRE(tiles * splits < (int64_t(1) << 31), "%s: too many elements", call.who);
-  auto kernel = mx_linear_kernel<NT, DUAL>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+  auto kernel = mx_linear_kernel<KIND, NT, DUAL>;
+  static std::atomic<bool> allowed[kMaxDevices];
+  cudaError_t err = allow_shared_memory(kernel, allowed, call.device);
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(unsigned(tiles * splits));
   config.blockDim = dim3(kLinThreads);
@@ -775,12 +819,9 @@ int launch_pairs(const LinearCall& call, int sms) {
   const int steps = int(mx_steps(call.cols));
   PairMaps maps;
   PairParams p;
-  p.out = call.out;
-  p.out_scales = static_cast<uint8_t*>(call.out_scales);
+  p.out = Output{call.out, static_cast<uint8_t*>(call.out_scales), call.features, (call.features + 127) / 128};
   p.rows = call.rows;
-  p.features = call.features;
   p.steps = steps;
-  p.w_tiles = (call.features + 127) / 128;
   p.pair_tiles = (call.features + 255) / 256;
   const int64_t tiles = (call.rows + kPairRows - 1) / kPairRows * p.pair_tiles;
   p.units = tiles * (DUAL ? 2 : 1);
@@ -790,17 +831,22 @@ int launch_pairs(const LinearCall& call, int sms) {
             uint32_t(kPairRows / 8) << 17 | 1u << 23 | uint32_t(256 / 16) << 24;
   bool ok = make_map(&maps.x, call.x.codes, call.x.format, call.rows, steps, kPairRows / 2) &&
             make_scale_map(&maps.x_scales, call.x.scales, call.rows, steps);
-  for (int i = 0; i < 2; ++i) {
-    const Operand& w = call.w[DUAL ? i : 0];
+  for (int i = 0; i < (DUAL ? 2 : 1); ++i) {
+    const Operand& w = call.w[i];
     ok = ok && make_map(&maps.w[i], w.codes, w.format, call.features, steps, 128) &&
          make_scale_map(&maps.w_scales[i], w.scales, call.features, steps);
   }
+  if (!DUAL) {
+    maps.w[1] = maps.w[0];
+    maps.w_scales[1] = maps.w_scales[0];
+  }
   FL_REQUIRE(ok, "%s: the operands cannot be described as tensor maps", call.who);
-  FL_REQUIRE(int64_t(p.w_tiles + 2) * steps < (int64_t(1) << 31) &&
+  FL_REQUIRE(int64_t(p.out.w_tiles + 2) * steps < (int64_t(1) << 31) &&
                  (call.rows / kMxTileRows + kPairXTiles + 1) * steps < (int64_t(1) << 31),
              "%s: too many elements", call.who);
   auto kernel = mx_linear_pair_kernel<KIND, DUAL>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+  static std::atomic<bool> allowed[kMaxDevices];
+  cudaError_t err = allow_shared_memory(kernel, allowed, call.device);
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(unsigned(2 * std::min<int64_t>(tiles, sms / 2)));
   config.blockDim = dim3(kPairThreads);
@@ -821,40 +867,76 @@ int launch_pairs(const LinearCall& call, int sms) {
   return FL_OK;
 }
 
-template <bool DUAL>
-int launch_pairs_of_kind(const LinearCall& call, int sms) {
-  switch (call.out_kind) {
-    case kOutBf16: return launch_pairs<kOutBf16, DUAL>(call, sms);
-    case kOutF16: return launch_pairs<kOutF16, DUAL>(call, sms);
-    case kOutF32: return launch_pairs<kOutF32, DUAL>(call, sms);
-    default: break;
-  }
-  if constexpr (DUAL) {
-    return call.out_kind == kOutFp8 ? launch_pairs<kOutFp8, true>(call, sms) : launch_pairs<kOutFp4, true>(call, sms);
-  } else {
-    FL_REQUIRE(false, "%s: unknown output type", call.who);
-  }
+// Multiprocessors of a device and, for every cluster size, how many clusters of CTAs that fill an SM each run
+// at once (the GPU's processor groups do not divide evenly).
+struct Device {
+  int sms;
+  int clusters[kMaxSplits + 1];
+};
+const Device& device_limits(int device) {
+  static Device limits[kMaxDevices];
+  static std::once_flag once[kMaxDevices];
+  std::call_once(once[device], [device] {
+    Device& d = limits[device];
+    d.sms = 0;
+    if (cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || d.sms <= 0) d.sms = 148;
+    auto kernel = mx_linear_kernel<kOutBf16, 16, false>;
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+    for (int size = 1; size <= kMaxSplits; ++size) {
+      cudaLaunchConfig_t config{};
+      config.gridDim = dim3(unsigned(size));
+      config.blockDim = dim3(kLinThreads);
+      config.dynamicSmemBytes = kSmemLimit;
+      cudaLaunchAttribute attribute;
+      attribute.id = cudaLaunchAttributeClusterDimension;
+      attribute.val.clusterDim.x = size;
+      attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+      config.attrs = &attribute;
+      config.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&d.clusters[size], kernel, &config) != cudaSuccess) d.clusters[size] = 0;
+    }
+    cudaGetLastError();
+  });
+  return limits[device];
+}
+
+template <int KIND, bool DUAL>
+int choose_linear(const LinearCall& call) {
+  const Device& device = device_limits(call.device);
+  const int sms = device.sms;
+  const int steps = int(mx_steps(call.cols));
+  const int64_t w_tiles = (call.features + 127) / 128;
+  // The widest split whose clusters all run at once: one that has to wait doubles the call.  MEASURED
+  auto splits_for = [&](int nt) {
+    const int64_t tiles = (call.rows + nt - 1) / nt * w_tiles;
+    int splits = std::min(kMaxSplits, steps);
+    while (splits > 1 && tiles > device.clusters[splits]) --splits;
+    return splits;
+  };
+  if (call.rows <= 16) return launch_linear<KIND, 16, DUAL>(call, splits_for(16), kMaxStages);
+  if (call.rows <= 32) return launch_linear<KIND, 32, DUAL>(call, splits_for(32), kMaxStages);
+  if (call.rows <= 64) return launch_linear<KIND, 64, DUAL>(call, splits_for(64), kMaxStages);
+  if ((call.rows + kPairRows - 1) / kPairRows * ((call.features + 255) / 256) >= sms / 2)
+    return launch_pairs<KIND, DUAL>(call, sms);
+  constexpr int kTile = DUAL ? 64 : 128;
+  return launch_linear<KIND, kTile, DUAL>(call, splits_for(kTile), kMaxStages);
 }
 
 template <bool DUAL>
-int choose_linear(const LinearCall& call) {
-  int device = 0;
-  cudaGetDevice(&device);
-  const int sms = sm_count(device);
-  const int steps = int(mx_steps(call.cols));
-  const int64_t w_tiles = (call.features + 127) / 128;
-  auto splits_for = [&](int nt) {
-    const int64_t tiles = (call.rows + nt - 1) / nt * w_tiles;
-    int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= sms && splits * 2 <= steps) splits *= 2;
-    return splits;
-  };
-  if (call.rows <= 16) return launch_linear<16, DUAL>(call, splits_for(16));
-  if (call.rows <= 32) return launch_linear<32, DUAL>(call, splits_for(32));
-  if (call.rows <= 64) return launch_linear<64, DUAL>(call, splits_for(64));
-  if ((call.rows + kPairRows - 1) / kPairRows * ((call.features + 255) / 256) >= sms / 2)
-    return launch_pairs_of_kind<DUAL>(call, sms);
-  return launch_linear<128, DUAL>(call, splits_for(128));
+int run_linear(LinearCall call) {
+  FL_REQUIRE(cudaGetDevice(&call.device) == cudaSuccess && call.device >= 0 && call.device < kMaxDevices,
+             "%s: no current device", call.who);
+  switch (call.out_kind) {
+    case kOutBf16: return choose_linear<kOutBf16, DUAL>(call);
+    case kOutF16: return choose_linear<kOutF16, DUAL>(call);
+    case kOutF32: return choose_linear<kOutF32, DUAL>(call);
+    default: break;
+  }
+  if constexpr (DUAL) {
+    return call.out_kind == kOutFp8 ? choose_linear<kOutFp8, true>(call) : choose_linear<kOutFp4, true>(call);
+  } else {
+    FL_REQUIRE(false, "%s: unknown output type", call.who);
+  }
 }
 
 int check_operand(const char* who, const char* name, const Operand& o) {
@@ -878,11 +960,11 @@ extern "C" int fl_mx_linear(const void* x_codes, const void* x_scales, int32_t x
   FL_REQUIRE(out_dtype >= kOutBf16 && out_dtype <= kOutF32, "%s: unknown output type", who);
   if (rows == 0) return FL_OK;
   LinearCall call{{x_codes, x_scales, x_format}, {{w_codes, w_scales, w_format}, {w_codes, w_scales, w_format}}, rows,
-                  in_features, out_features, out_dtype, out, nullptr, static_cast<cudaStream_t>(stream), who};
+                  in_features, out_features, out_dtype, out, nullptr, static_cast<cudaStream_t>(stream), who, 0};
   if (int rc = check_operand(who, "x", call.x)) return rc;
   if (int rc = check_operand(who, "weight", call.w[0])) return rc;
   FL_REQUIRE(out && aligned16(out), "%s: out must be given, 16-byte aligned", who);
-  return choose_linear<false>(call);
+  return run_linear<false>(call);
 }
 
 extern "C" int fl_mx_linear_swiglu(const void* x_codes, const void* x_scales, int32_t x_format, const void* gate_codes,
@@ -897,12 +979,12 @@ extern "C" int fl_mx_linear_swiglu(const void* x_codes, const void* x_scales, in
   if (rows == 0) return FL_OK;
   const int kind = out_scales == nullptr ? out_dtype : out_format == FL_MX_FP8 ? int(kOutFp8) : int(kOutFp4);
   LinearCall call{{x_codes, x_scales, x_format}, {{gate_codes, gate_scales, w_format}, {up_codes, up_scales, w_format}},
-                  rows, in_features, out_features, kind, out, out_scales, static_cast<cudaStream_t>(stream), who};
+                  rows, in_features, out_features, kind, out, out_scales, static_cast<cudaStream_t>(stream), who, 0};
   if (int rc = check_operand(who, "x", call.x)) return rc;
   if (int rc = check_operand(who, "gate", call.w[0])) return rc;
   if (int rc = check_operand(who, "up", call.w[1])) return rc;
   FL_REQUIRE(out && aligned16(out) && aligned16(out_scales), "%s: outputs must be given, 16-byte aligned", who);
-  return choose_linear<true>(call);
+  return run_linear<true>(call);
 }
 
 extern "C" int fl_mx_status(int32_t* status, int32_t reset, fl_cuda_stream stream) {

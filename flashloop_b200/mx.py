@@ -10,10 +10,13 @@ instead.  Inference only: no gradient is recorded, and inputs that require one a
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import torch
 
 from . import _native
+
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: a Stream object costs 2 us
 
 FORMATS = {"mxfp8": 0, "mxfp4": 1}
 MAX_NORM_WIDTH = 8192
@@ -46,16 +49,15 @@ class MXTensor:
     (:func:`scales_shape`, rows past the last zero; byte b stands for 2^(b - 127), 255 for NaN) of
     ``shape``, whose leading dimensions are the rows.  The tensors are held, not copied."""
 
-    __slots__ = ("codes", "scales", "shape", "format", "rows", "cols", "_code")
+    __slots__ = ("shape", "format", "rows", "cols", "device", "codes_ptr", "scales_ptr", "_code", "_codes", "_scales",
+                 "_both")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, format: str) -> None:
         shape = tuple(int(v) for v in shape)
         if not shape or min(shape) < 0 or shape[-1] <= 0:
             raise ValueError("a microscaled tensor needs at least one dimension and a positive last one")
-        rows = 1
-        for v in shape[:-1]:
-            rows *= v
-        code = _format_code(format)
+        rows = math.prod(shape[:-1])
+        self._code = _format_code(format)
         for t, want, name in ((codes, codes_shape(rows, shape[-1], format), "codes"),
                               (scales, scales_shape(rows, shape[-1]), "scales")):
             if t.dtype != torch.uint8 or not t.is_contiguous():
@@ -64,28 +66,52 @@ class MXTensor:
                 raise ValueError(f"{name} of {shape} in {format} must be {want}, got {tuple(t.shape)}")
         if codes.device != scales.device:
             raise ValueError("codes and scales must be on one device")
-        self._set(codes, scales, shape, format, rows, code)
-
-    def _set(self, codes, scales, shape, format, rows, code) -> None:
-        self.codes, self.scales, self.shape, self.format = codes, scales, shape, format
-        self.rows, self.cols, self._code = rows, shape[-1], code
+        self.shape, self.format, self.rows, self.cols, self.device = shape, format, rows, shape[-1], codes.device
+        self._codes, self._scales, self._both = codes, scales, None
+        self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
-    def _empty(cls, shape: tuple, rows: int, format: str, device: torch.device) -> "MXTensor":
+    def _empty(cls, shape: tuple, rows: int, format: str, like: torch.Tensor) -> "MXTensor":
+        """Uninitialised, on the device of ``like``: codes and then scales in one allocation."""
+
         self = object.__new__(cls)
-        cols, code = shape[-1], _format_code(format)
-        steps = (cols + 127) // 128
-        codes = torch.empty((rows, steps * (64 if code else 128)), dtype=torch.uint8, device=device)
-        scales = torch.empty(((rows + 127) // 128, steps, 32, 4, 4), dtype=torch.uint8, device=device)
-        self._set(codes, scales, shape, format, rows, code)
+        cols = shape[-1]
+        code = self._code = _format_code(format)
+        steps = (cols + 127) >> 7
+        at = (rows * steps * (64 if code else 128) + 511) & ~511
+        both = like.new_empty(at + ((rows + 127) >> 7) * steps * 512, dtype=torch.uint8)
+        self.shape, self.format, self.rows, self.cols, self.device = shape, format, rows, cols, like.device
+        self._codes = self._scales = None
+        self._both = both
+        self.codes_ptr = both.data_ptr()
+        self.scales_ptr = self.codes_ptr + at
         return self
 
+    def _any(self) -> torch.Tensor:
+        """A tensor of this one's device, to allocate beside."""
+
+        return self._codes if self._both is None else self._both
+
     @property
-    def device(self) -> torch.device:
-        return self.codes.device
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            rows, width = codes_shape(self.rows, self.cols, self.format)
+            self._codes = self._both.as_strided((rows, width), (width, 1))
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            tiles, steps = (self.rows + 127) >> 7, (self.cols + 127) >> 7
+            self._scales = self._both.as_strided((tiles, steps, 32, 4, 4), (steps * 512, 512, 16, 4, 1),
+                                                 self.scales_ptr - self.codes_ptr)
+        return self._scales
+
+    def __reduce__(self):  # copies and pickles hold tensors of their own
+        return MXTensor, (self.codes, self.scales, self.shape, self.format)
 
     def __repr__(self) -> str:
-        return f"MXTensor(shape={self.shape}, format={self.format!r}, device={self.codes.device})"
+        return f"MXTensor(shape={self.shape}, format={self.format!r}, device={self.device})"
 
     def nbytes(self) -> int:
         return self.codes.numel() + self.scales.numel()
@@ -100,43 +126,45 @@ class MXTensor:
 
         if dtype not in _native.DTYPE_CODES:
             raise TypeError("dequantize gives bfloat16, float16 or float32")
-        device = self.codes.device
-        _native.require_cuda(self.codes)
-        out = torch.empty(self.shape, dtype=dtype, device=device)
-        _call(device, "fl_mx_dequantize", self.codes.data_ptr(), self.scales.data_ptr(), self._code, self.rows, self.cols,
+        _require_cuda(self.device)
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        _call(self.device, "fl_mx_dequantize", self.codes_ptr, self.scales_ptr, self._code, self.rows, self.cols,
               out.data_ptr(), _native.DTYPE_CODES[dtype])
         return out
+
+
+def _require_cuda(device: torch.device) -> None:
+    if device.type != "cuda":
+        raise RuntimeError("flashloop_b200 kernels need CUDA tensors (there is no CPU fallback)")
 
 
 def _call(device: torch.device, name: str, *args) -> None:
     """One entry point on the current stream of ``device`` (made the current device for the call)."""
 
     function = getattr(_native.load(), name)
-    if device.index == torch.cuda.current_device():
-        status = function(*args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = function(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            status = function(*args, torch.cuda.current_stream(device).cuda_stream)
+            status = function(*args, _raw_stream(index))
     if status:
         _native.check(status, name)
 
 
-def _values(*tensors: torch.Tensor | None) -> None:
+def _values(x: torch.Tensor, *others: torch.Tensor | None) -> None:
     """Floating-point CUDA inputs of one device that need no gradient."""
 
-    device = None
-    for t in tensors:
-        if t is None:
-            continue
-        if t.dtype not in _native.DTYPE_CODES:
-            raise TypeError("microscaled operators take bfloat16, float16 or float32")
-        _native.require_cuda(t)
-        if device is None:
-            device = t.device
-        elif t.device != device:
+    if x.dtype not in _native.DTYPE_CODES:
+        raise TypeError("microscaled operators take bfloat16, float16 or float32")
+    device = x.device
+    _require_cuda(device)
+    for t in others:
+        if t is not None and t.device != device:
+            _require_cuda(t.device)
             raise ValueError("all operands must be on one device")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("microscaled operators record no gradient: call them under torch.no_grad()")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, *others)):
+        raise RuntimeError("microscaled operators record no gradient: call them under torch.no_grad()")
 
 
 def mx_quantize(x: torch.Tensor, format: str = "mxfp8") -> MXTensor:
@@ -155,9 +183,9 @@ def mx_quantize(x: torch.Tensor, format: str = "mxfp8") -> MXTensor:
         if (x.stride(1) != 1 and cols > 1) or (x.stride(0) < cols and x.shape[0] > 1):
             x = x.contiguous()
     rows = x.shape[0]
-    q = MXTensor._empty(shape, rows, format, x.device)
+    q = MXTensor._empty(shape, rows, format, x)
     _call(x.device, "fl_mx_quantize", x.data_ptr(), _native.DTYPE_CODES[x.dtype], rows, cols, x.stride(0), q._code,
-          q.codes.data_ptr(), q.scales.data_ptr())
+          q.codes_ptr, q.scales_ptr)
     return q
 
 
@@ -188,13 +216,13 @@ def mx_rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: t
     residual = None if residual is None else residual.contiguous()
     addend = None if addend is None else addend.contiguous()
     rows = x.numel() // width
-    q = MXTensor._empty(shape, rows, format, x.device)
+    q = MXTensor._empty(shape, rows, format, x)
     hidden = None if weight2 is None else torch.empty_like(x)
     total = torch.empty_like(x) if want_sum else None
     ptr = _native.ptr
     _call(x.device, "fl_rmsnorm_mx", x.data_ptr(), ptr(addend), ptr(residual), weight.data_ptr(), eps, ptr(weight2), eps2,
-          _native.DTYPE_CODES[x.dtype], rows, width, q._code, ptr(total), ptr(hidden), q.codes.data_ptr(),
-          q.scales.data_ptr())
+          _native.DTYPE_CODES[x.dtype], rows, width, q._code, ptr(total), ptr(hidden), q.codes_ptr,
+          q.scales_ptr)
     return q, hidden, total
 
 
@@ -209,8 +237,9 @@ def _operand(x, weight: MXTensor) -> MXTensor:
         raise TypeError("x must be an MXTensor or a tensor to quantise")
     if x.cols != weight.cols:
         raise ValueError("x and weight do not match")
-    _native.require_cuda(x.codes, weight.codes)
-    if x.codes.device != weight.codes.device:
+    _require_cuda(x.device)
+    if x.device != weight.device:
+        _require_cuda(weight.device)
         raise ValueError("all operands must be on one device")
     return x
 
@@ -223,13 +252,11 @@ def mx_linear(x, weight: MXTensor, *, out_dtype: torch.dtype = torch.bfloat16) -
     x = _operand(x, weight)
     if out_dtype not in _native.DTYPE_CODES:
         raise TypeError("out_dtype is bfloat16, float16 or float32")
-    features = weight.shape[0]
-    device = x.codes.device
-    out = torch.empty((*x.shape[:-1], features), dtype=out_dtype, device=device)
-    if out.numel():
-        _call(device, "fl_mx_linear", x.codes.data_ptr(), x.scales.data_ptr(), x._code, weight.codes.data_ptr(),
-              weight.scales.data_ptr(), weight._code, x.rows, features, x.cols, out.data_ptr(),
-              _native.DTYPE_CODES[out_dtype])
+    features = weight.rows
+    out = x._any().new_empty((*x.shape[:-1], features), dtype=out_dtype)
+    if x.rows and features:
+        _call(x.device, "fl_mx_linear", x.codes_ptr, x.scales_ptr, x._code, weight.codes_ptr, weight.scales_ptr,
+              weight._code, x.rows, features, x.cols, out.data_ptr(), _native.DTYPE_CODES[out_dtype])
     return out
 
 
@@ -243,23 +270,21 @@ def mx_linear_swiglu(x, gate: MXTensor, up: MXTensor, *, out_dtype: torch.dtype 
     _operand(x, up)
     if gate.shape != up.shape or gate.format != up.format:
         raise ValueError("gate and up must agree in shape and format")
-    features = gate.shape[0]
-    device = x.codes.device
+    features = gate.rows
     shape = (*x.shape[:-1], features)
     if out_format is not None:
         if features == 0:
             raise ValueError("a microscaled result needs at least one feature")
-        out = MXTensor._empty(shape, x.rows, out_format, device)
-        target, dtype, fmt, scales = out.codes, 0, out._code, out.scales.data_ptr()
+        out = MXTensor._empty(shape, x.rows, out_format, x._any())
+        target, dtype, fmt, scales = out.codes_ptr, 0, out._code, out.scales_ptr
     else:
         if out_dtype not in _native.DTYPE_CODES:
             raise TypeError("out_dtype is bfloat16, float16 or float32")
-        out = target = torch.empty(shape, dtype=out_dtype, device=device)
-        dtype, fmt, scales = _native.DTYPE_CODES[out_dtype], 0, None
-    if target.numel():
-        _call(device, "fl_mx_linear_swiglu", x.codes.data_ptr(), x.scales.data_ptr(), x._code, gate.codes.data_ptr(),
-              gate.scales.data_ptr(), up.codes.data_ptr(), up.scales.data_ptr(), gate._code, x.rows, features, x.cols,
-              target.data_ptr(), dtype, fmt, scales)
+        out = x._any().new_empty(shape, dtype=out_dtype)
+        target, dtype, fmt, scales = out.data_ptr(), _native.DTYPE_CODES[out_dtype], 0, None
+    if x.rows and features:
+        _call(x.device, "fl_mx_linear_swiglu", x.codes_ptr, x.scales_ptr, x._code, gate.codes_ptr, gate.scales_ptr,
+              up.codes_ptr, up.scales_ptr, gate._code, x.rows, features, x.cols, target, dtype, fmt, scales)
     return out
 
 
