@@ -11,69 +11,97 @@ constexpr int kMxThreads = 256;
 
 // Sixteen lanes take one step (128 elements) of a row, eight elements each: four lanes share a block,
 // whose largest magnitude takes two shuffles, and the four scale bytes of the step leave as one word.
-template <typename T, int FORMAT, bool VEC>
+// A CTA takes UNROLL * 16 consecutive steps and asks for all of its elements before it uses any.
+template <typename T, int FORMAT, bool VEC, int UNROLL>
 __global__ void __launch_bounds__(kMxThreads)
-quantize_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t row_stride, uint32_t steps, uint32_t units,
+quantize_kernel(const T* __restrict__ x, uint32_t rows, int cols, int64_t row_stride, uint32_t steps, uint32_t units,
                 uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  const uint32_t unit = blockIdx.x * (kMxThreads / 16) + threadIdx.x / 16;
+  const uint32_t first = blockIdx.x * (UNROLL * kMxThreads / 16) + threadIdx.x / 16;
   const int lane = threadIdx.x & 15;
-  const uint32_t row = unit / steps, step = unit - row * steps;
-  const bool live = unit < units && row < rows;
-  float v[8] = {};
-  const int e = int(step) * kMxStep + lane * 8;
-  if (live) load8<T, VEC>(x + int64_t(row) * row_stride + e, cols - e, v);
-  uint32_t out[2];
-  const uint32_t word = mx_join_scales(mx_encode8<FORMAT>(v, out));
-  if (live) store_codes<FORMAT>(codes + int64_t(row) * steps * (FORMAT == FL_MX_FP8 ? kMxStep : kMxStep / 2), e, out);
-  // units past the last row belong to the last scale tile: their values are zero, and so is the word
-  if (unit < units && lane == 0) *reinterpret_cast<uint32_t*>(scales + mx_scale_offset(row, step, steps)) = word;
+  Raw8<T> raw[UNROLL];
+  uint32_t row[UNROLL];
+  int e[UNROLL];
+#pragma unroll
+  for (int i = 0; i < UNROLL; ++i) {
+    const uint32_t unit = first + i * (kMxThreads / 16);
+    row[i] = unit / steps;
+    e[i] = int(unit - row[i] * steps) * kMxStep + lane * 8;
+    raw[i].template load<VEC>(x + int64_t(row[i]) * row_stride + e[i], unit < units && row[i] < rows ? cols - e[i] : 0);
+  }
+#pragma unroll
+  for (int i = 0; i < UNROLL; ++i) {
+    const uint32_t unit = first + i * (kMxThreads / 16);
+    float v[8];
+    raw[i].unpack(v);
+    uint32_t out[2];
+    const uint32_t word = mx_join_scales(mx_encode8<FORMAT>(v, out));
+    if (unit >= units) continue;
+    if (row[i] < rows) {
+      store_codes<FORMAT>(codes + int64_t(unit) * (FORMAT == FL_MX_FP8 ? kMxStep : kMxStep / 2), lane * 8, out);
+    }
+    // steps past the last row belong to the last scale tile: their values are zero, and so is the word
+    if (lane == 0)
+      *reinterpret_cast<uint32_t*>(scales + mx_scale_offset(row[i], uint32_t(e[i]) / kMxStep, steps)) = word;
+  }
 }
 
-// Eight elements of a row per thread.
-template <typename T, int FORMAT>
+// Eight elements of a row per thread and round.
+template <typename T, int FORMAT, int UNROLL>
 __global__ void __launch_bounds__(kMxThreads)
 dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int cols, uint32_t steps,
                   uint32_t units, T* __restrict__ out) {
-  const uint32_t unit = blockIdx.x * (kMxThreads / 16) + threadIdx.x / 16;
-  if (unit >= units) return;
-  const uint32_t row = unit / steps, step = unit - row * steps;
+  const uint32_t first = blockIdx.x * (UNROLL * kMxThreads / 16) + threadIdx.x / 16;
   const int lane = threadIdx.x & 15;
-  const int e = int(step) * kMxStep + lane * 8;
-  if (e >= cols) return;
-  const float scale = mx_scale_value(__ldg(scales + mx_scale_offset(row, step, steps) + lane / 4));
-  const uint8_t* src = codes + int64_t(unit) * (FORMAT == FL_MX_FP8 ? kMxStep : kMxStep / 2);
-  float v[8];
-  if (FORMAT == FL_MX_FP8) {
-    const uint2 w = ldg64(src + lane * 8);
+  uint2 word[UNROLL] = {};
+  uint32_t byte[UNROLL] = {};
+  uint32_t row[UNROLL];
+  int e[UNROLL];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint16_t pair = uint16_t((k < 2 ? w.x : w.y) >> (16 * (k & 1)));
-      uint32_t h;
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(pair));
-      const float2 f = __half22float2(as_half2(h));
-      v[2 * k] = f.x * scale;
-      v[2 * k + 1] = f.y * scale;
-    }
-  } else {
-    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(src + lane * 4));
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint32_t h;
-      asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"((w >> (8 * k)) & 255u));
-      const float2 f = __half22float2(as_half2(h));
-      v[2 * k] = f.x * scale;
-      v[2 * k + 1] = f.y * scale;
+  for (int i = 0; i < UNROLL; ++i) {
+    const uint32_t unit = first + i * (kMxThreads / 16);
+    row[i] = unit / steps;
+    const uint32_t step = unit - row[i] * steps;
+    e[i] = unit < units ? int(step) * kMxStep + lane * 8 : cols;
+    if (e[i] < cols) {
+      const uint8_t* src = codes + int64_t(unit) * (FORMAT == FL_MX_FP8 ? kMxStep : kMxStep / 2);
+      if (FORMAT == FL_MX_FP8) {
+        word[i] = ldg64(src + lane * 8);
+      } else {
+        word[i].x = __ldg(reinterpret_cast<const uint32_t*>(src + lane * 4));
+      }
+      byte[i] = __ldg(scales + mx_scale_offset(row[i], step, steps) + lane / 4);
     }
   }
-  T* dst = out + int64_t(row) * cols + e;
-  if (cols % 8 == 0) {
-    store8<T, true>(dst, cols - e, v);
-  } else {
-    store8<T, false>(dst, cols - e, v);
+#pragma unroll
+  for (int i = 0; i < UNROLL; ++i) {
+    if (e[i] >= cols) continue;
+    const float scale = mx_scale_value(byte[i]);
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t h;
+      if (FORMAT == FL_MX_FP8) {
+        const uint16_t pair = uint16_t((k < 2 ? word[i].x : word[i].y) >> (16 * (k & 1)));
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(pair));
+      } else {
+        asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"((word[i].x >> (8 * k)) & 255u));
+      }
+      const float2 f = __half22float2(as_half2(h));
+      v[2 * k] = f.x * scale;
+      v[2 * k + 1] = f.y * scale;
+    }
+    T* dst = out + int64_t(row[i]) * cols + e[i];
+    if (cols % 8 == 0) {
+      store8<T, true>(dst, cols - e[i], v);
+    } else {
+      store8<T, false>(dst, cols - e[i], v);
+    }
   }
 }
 
-constexpr int kNormChunks = 4;  // eight elements per thread and chunk: rows up to 8192 wide
+// Rows up to 8192 wide: eight warps of four chunks of eight elements per thread, four of eight chunks.
+constexpr int kMaxNormWidth = 8192;
+constexpr int64_t kManyRows = 148 * 8;
 
 template <typename T>
 struct MxNormParams {
@@ -92,94 +120,151 @@ struct MxNormParams {
   uint8_t* scales;
 };
 
-__device__ __forceinline__ float cta_sum(float v, float* s_part) {
+// Sum over the warps of a row; every thread gets it.
+template <int WARPS>
+__device__ __forceinline__ float row_sum(float v, float* s_part) {
   v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = v;
+  if (WARPS == 1) return v;
+  const int warp = threadIdx.x >> 5, first = warp / WARPS * WARPS;
+  __syncthreads();  // s_part may still be read from the previous sum
+  if ((threadIdx.x & 31) == 0) s_part[warp] = v;
   __syncthreads();
   float total = 0.f;
 #pragma unroll
-  for (int w = 0; w < kMxThreads / 32; ++w) total += s_part[w];
+  for (int w = 0; w < WARPS; ++w) total += s_part[first + w];
   return total;
+}
+
+// 1 / sqrt(mean + eps): the hardware's root and one Newton step, so that the float32 result carries the rounding
+// of its products only.
+__device__ __forceinline__ float inverse_root(float sum, int width, float eps) {
+  const float m = sum / float(width) + eps;
+  const float y = rsqrtf(m);
+  const float r = fmaf(-m * y, y, 1.f);
+  return isfinite(y) ? fmaf(0.5f * y, r, y) : y;
 }
 
 // s = round(addend + x) or x;  n = weight * s * rsqrt(mean(s^2) + eps).  Without weight2 the codes are
 // those of n; with it hidden = round([residual +] n) and the codes are those of weight2 * hidden *
 // rsqrt(mean(hidden^2) + eps2).  Everything between two stored tensors stays in float32.
-template <typename T, int FORMAT, bool VEC>
+//
+// WARPS warps share a row and hold it in registers, CHUNKS times eight elements per thread; what the
+// row needs from memory is requested before the first sum.  Many rows take few warps each, with no
+// barrier but that of the warp: bound by memory (MEASURED).  Few rows take eight: bound by latency.
+template <typename T, int FORMAT, bool VEC, int WARPS, int CHUNKS>
 __global__ void __launch_bounds__(kMxThreads) norm_mx_kernel(const MxNormParams<T> p) {
+  constexpr int kRowThreads = WARPS * 32, kRows = kMxThreads / kRowThreads;
   __shared__ float s_part[kMxThreads / 32];
-  const int64_t row = blockIdx.x;
+  const int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / kRowThreads;
+  const int thread = threadIdx.x % kRowThreads;
+  const bool live = row < p.rows;
   const int64_t base = row * p.width;
-  float v[kNormChunks][8];
+  Raw8<T> raw_x[CHUNKS], raw_a[CHUNKS], raw_r[CHUNKS];
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int e = (c * kRowThreads + thread) * 8, n = live ? p.width - e : 0;
+    raw_x[c].template load<VEC>(p.x + base + e, n);
+    if (p.addend) raw_a[c].template load<VEC>(p.addend + base + e, n);
+    if (p.residual) raw_r[c].template load<VEC>(p.residual + base + e, n);
+  }
+  float v[CHUNKS][8];
   float sq = 0.f;
 #pragma unroll
-  for (int c = 0; c < kNormChunks; ++c) {
-    const int e = (c * kMxThreads + threadIdx.x) * 8;
-    const int n = p.width - e;
-    if (n <= 0) continue;
-    load8<T, VEC>(p.x + base + e, n, v[c]);
+  for (int c = 0; c < CHUNKS; ++c) {
+    raw_x[c].unpack(v[c]);
     if (p.addend) {
+      const int e = (c * kRowThreads + thread) * 8, n = live ? p.width - e : 0;
       float a[8];
-      load8<T, VEC>(p.addend + base + e, n, a);
+      raw_a[c].unpack(a);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[c][k] += a[k];
-      store8<T, VEC>(p.sum_out ? p.sum_out + base + e : nullptr, n, v[c]);
+      store8<T, VEC>(p.sum_out && n > 0 ? p.sum_out + base + e : nullptr, n, v[c]);
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) sq = fmaf(v[c][k], v[c][k], sq);
   }
-  float inv = rsqrtf(cta_sum(sq, s_part) / float(p.width) + p.eps);
+  float inv = inverse_root(row_sum<WARPS>(sq, s_part), p.width, p.eps);
   sq = 0.f;
 #pragma unroll
-  for (int c = 0; c < kNormChunks; ++c) {
-    const int e = (c * kMxThreads + threadIdx.x) * 8;
-    const int n = p.width - e;
-    if (n <= 0) continue;
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int e = (c * kRowThreads + thread) * 8, n = live ? p.width - e : 0;
     float w[8];
-    load8<T, VEC>(p.weight + e, n, w);
+    load8<T, VEC>(p.weight + e, p.width - e, w);
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[c][k] = w[k] * (v[c][k] * inv);
     if (p.weight2) {
       if (p.residual) {
         float r[8];
-        load8<T, VEC>(p.residual + base + e, n, r);
+        raw_r[c].unpack(r);
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[c][k] += r[k];
       }
-      store8<T, VEC>(p.hidden + base + e, n, v[c]);
+      store8<T, VEC>(n > 0 ? p.hidden + base + e : nullptr, n, v[c]);
 #pragma unroll
       for (int k = 0; k < 8; ++k) sq = fmaf(v[c][k], v[c][k], sq);
     }
   }
-  if (p.weight2) inv = rsqrtf(cta_sum(sq, s_part) / float(p.width) + p.eps2);
+  if (p.weight2) inv = inverse_root(row_sum<WARPS>(sq, s_part), p.width, p.eps2);
+  uint8_t* codes = p.codes + row * p.steps * (FORMAT == FL_MX_FP8 ? kMxStep : kMxStep / 2);
+  const bool one_group = p.rows <= 32;  // a row's word is then the only one of its sixteen bytes
 #pragma unroll
-  for (int c = 0; c < kNormChunks; ++c) {
-    const uint32_t step = (c * kMxThreads + threadIdx.x) / 16;
-    if (c * (kMxThreads / 16) >= int(p.steps)) continue;  // the same for the whole CTA
-    const int e = (c * kMxThreads + threadIdx.x) * 8;
-    const int n = p.width - e;
-    if (n <= 0) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[c][k] = 0.f;
-    } else if (p.weight2) {
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int e = (c * kRowThreads + thread) * 8;
+    const uint32_t step = uint32_t(e) / kMxStep;
+    if (c * kRowThreads * 8 >= p.width) continue;  // the same for the whole CTA
+    if (p.weight2) {
       float w[8];
-      load8<T, VEC>(p.weight2 + e, n, w);
+      load8<T, VEC>(p.weight2 + e, p.width - e, w);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[c][k] = w[k] * (v[c][k] * inv);
     }
+    if (e >= p.width) {  // padding is zero also where the row is not finite
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[c][k] = 0.f;
+    }
     uint32_t out[2];
     const uint32_t word = mx_join_scales(mx_encode8<FORMAT>(v[c], out));
-    if (step < p.steps) {
-      store_codes<FORMAT>(p.codes + row * p.steps * (FORMAT == FL_MX_FP8 ? kMxStep : kMxStep / 2), e, out);
-      if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint32_t*>(p.scales + mx_scale_offset(row, step, p.steps)) = word;
+    if (live && step < p.steps) {
+      store_codes<FORMAT>(codes, e, out);
+      if ((threadIdx.x & 15) == 0) {
+        uint8_t* at = p.scales + mx_scale_offset(row, step, p.steps);
+        if (one_group) {
+          *reinterpret_cast<uint4*>(at) = make_uint4(word, 0u, 0u, 0u);
+        } else {
+          *reinterpret_cast<uint32_t*>(at) = word;
+        }
+      }
     }
   }
-  // rows of the last scale tile past the last row
-  const int64_t end = (p.rows + kMxTileRows - 1) / kMxTileRows * kMxTileRows;
-  for (int64_t r = row + p.rows; r < end; r += p.rows)
-    for (uint32_t step = threadIdx.x; step < p.steps; step += kMxThreads)
-      *reinterpret_cast<uint32_t*>(p.scales + mx_scale_offset(r, step, p.steps)) = 0u;
+  // rows of the last scale tile past the last row, shared out over all threads
+  const uint32_t threads = gridDim.x * kMxThreads, mine = blockIdx.x * kMxThreads + threadIdx.x;
+  if (one_group) {
+    const uint32_t empty = 32u - uint32_t(p.rows);  // sixteen-byte groups of a step that hold no row
+    for (uint32_t i = mine; i < empty * p.steps; i += threads)
+      *reinterpret_cast<uint4*>(p.scales + mx_scale_offset(p.rows + i / p.steps, i % p.steps, p.steps)) = make_uint4(0u, 0u, 0u, 0u);
+  } else {
+    const uint32_t empty = uint32_t(-p.rows & (kMxTileRows - 1));
+    for (uint32_t i = mine; i < empty * p.steps; i += threads)
+      *reinterpret_cast<uint32_t*>(p.scales + mx_scale_offset(p.rows + i / p.steps, i % p.steps, p.steps)) = 0u;
+  }
+}
+
+// Rounds per thread: four where that still leaves several CTAs to an SM, one below.
+constexpr int64_t kUnrollUnits = 148 * 8 * 64;
+
+template <typename T, int FORMAT, bool VEC>
+void launch_quantize(const T* x, int64_t rows, int32_t cols, int64_t stride, uint32_t steps, uint32_t units, void* codes,
+                     void* scales, cudaStream_t stream) {
+  uint8_t* c = static_cast<uint8_t*>(codes);
+  uint8_t* s = static_cast<uint8_t*>(scales);
+  constexpr int kUnits = kMxThreads / 16;
+  if (units >= kUnrollUnits) {
+    quantize_kernel<T, FORMAT, VEC, 4><<<(units + 4 * kUnits - 1) / (4 * kUnits), kMxThreads, 0, stream>>>(
+        x, uint32_t(rows), cols, stride, steps, units, c, s);
+  } else {
+    quantize_kernel<T, FORMAT, VEC, 1><<<(units + kUnits - 1) / kUnits, kMxThreads, 0, stream>>>(
+        x, uint32_t(rows), cols, stride, steps, units, c, s);
+  }
 }
 
 template <typename T, int FORMAT>
@@ -188,14 +273,11 @@ int launch_quantize(const void* x, int64_t rows, int32_t cols, int64_t stride, v
   const int64_t steps = mx_steps(cols);
   const int64_t units = (rows + kMxTileRows - 1) / kMxTileRows * kMxTileRows * steps;
   FL_REQUIRE(units < (int64_t(1) << 31), "fl_mx_quantize: too many elements");
-  const unsigned grid = unsigned((units + kMxThreads / 16 - 1) / (kMxThreads / 16));
   const T* src = static_cast<const T*>(x);
-  uint8_t* c = static_cast<uint8_t*>(codes);
-  uint8_t* s = static_cast<uint8_t*>(scales);
-  if (aligned16(x) && stride * sizeof(T) % 16 == 0) {
-    quantize_kernel<T, FORMAT, true><<<grid, kMxThreads, 0, stream>>>(src, rows, cols, stride, uint32_t(steps), uint32_t(units), c, s);
+  if (aligned16(x) && (stride * sizeof(T) % 16 == 0 || rows == 1)) {
+    launch_quantize<T, FORMAT, true>(src, rows, cols, stride, uint32_t(steps), uint32_t(units), codes, scales, stream);
   } else {
-    quantize_kernel<T, FORMAT, false><<<grid, kMxThreads, 0, stream>>>(src, rows, cols, stride, uint32_t(steps), uint32_t(units), c, s);
+    launch_quantize<T, FORMAT, false>(src, rows, cols, stride, uint32_t(steps), uint32_t(units), codes, scales, stream);
   }
   FL_CHECK_LAUNCH("fl_mx_quantize");
   return FL_OK;
@@ -206,10 +288,16 @@ int launch_dequantize(const void* codes, const void* scales, int64_t rows, int32
                       cudaStream_t stream) {
   const int64_t steps = mx_steps(cols), units = rows * steps;
   FL_REQUIRE(units < (int64_t(1) << 31), "fl_mx_dequantize: too many elements");
-  const unsigned grid = unsigned((units + kMxThreads / 16 - 1) / (kMxThreads / 16));
-  dequantize_kernel<T, FORMAT><<<grid, kMxThreads, 0, stream>>>(
-      static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), cols, uint32_t(steps), uint32_t(units),
-      static_cast<T*>(out));
+  constexpr int kUnits = kMxThreads / 16;
+  const uint8_t* c = static_cast<const uint8_t*>(codes);
+  const uint8_t* s = static_cast<const uint8_t*>(scales);
+  if (units >= kUnrollUnits) {
+    dequantize_kernel<T, FORMAT, 4><<<unsigned((units + 4 * kUnits - 1) / (4 * kUnits)), kMxThreads, 0, stream>>>(
+        c, s, cols, uint32_t(steps), uint32_t(units), static_cast<T*>(out));
+  } else {
+    dequantize_kernel<T, FORMAT, 1><<<unsigned((units + kUnits - 1) / kUnits), kMxThreads, 0, stream>>>(
+        c, s, cols, uint32_t(steps), uint32_t(units), static_cast<T*>(out));
+  }
   FL_CHECK_LAUNCH("fl_mx_dequantize");
   return FL_OK;
 }
@@ -221,6 +309,25 @@ struct NormArgs {
   int32_t width;
   void *sum_out, *hidden, *codes, *scales;
 };
+
+template <typename T, int FORMAT, bool VEC, int WARPS, int CHUNKS>
+void launch_norm_shape(const MxNormParams<T>& p, cudaStream_t stream) {
+  constexpr int kRows = kMxThreads / 32 / WARPS;
+  norm_mx_kernel<T, FORMAT, VEC, WARPS, CHUNKS><<<unsigned((p.rows + kRows - 1) / kRows), kMxThreads, 0, stream>>>(p);
+}
+
+// Warps to a row: as few as hold it once there are rows enough to fill the SMs, otherwise all eight of a CTA.
+template <typename T, int FORMAT, bool VEC>
+void launch_norm_rows(const MxNormParams<T>& p, cudaStream_t stream) {
+  const bool many = p.rows >= kManyRows;
+  if (many && p.width <= 512) return launch_norm_shape<T, FORMAT, VEC, 1, 2>(p, stream);
+  if (many && p.width <= 1024) return launch_norm_shape<T, FORMAT, VEC, 1, 4>(p, stream);
+  if (many && p.width <= 2048) return launch_norm_shape<T, FORMAT, VEC, 2, 4>(p, stream);
+  if (many && p.width <= 4096) return launch_norm_shape<T, FORMAT, VEC, 4, 4>(p, stream);
+  if (p.width <= 2048) return launch_norm_shape<T, FORMAT, VEC, 8, 1>(p, stream);
+  if (p.width <= 4096) return launch_norm_shape<T, FORMAT, VEC, 8, 2>(p, stream);
+  return launch_norm_shape<T, FORMAT, VEC, 8, 4>(p, stream);
+}
 
 template <typename T, int FORMAT>
 int launch_norm(const NormArgs& a, cudaStream_t stream) {
@@ -243,9 +350,9 @@ int launch_norm(const NormArgs& a, cudaStream_t stream) {
                    aligned16(a.weight2) && aligned16(a.sum_out) && aligned16(a.hidden) &&
                    a.width * sizeof(T) % 16 == 0;
   if (vec) {
-    norm_mx_kernel<T, FORMAT, true><<<unsigned(a.rows), kMxThreads, 0, stream>>>(p);
+    launch_norm_rows<T, FORMAT, true>(p, stream);
   } else {
-    norm_mx_kernel<T, FORMAT, false><<<unsigned(a.rows), kMxThreads, 0, stream>>>(p);
+    launch_norm_rows<T, FORMAT, false>(p, stream);
   }
   FL_CHECK_LAUNCH("fl_rmsnorm_mx");
   return FL_OK;
@@ -335,8 +442,8 @@ extern "C" int fl_rmsnorm_mx(const void* x, const void* addend, const void* resi
                              fl_cuda_stream stream) {
   const char* who = "fl_rmsnorm_mx";
   FL_REQUIRE(dtype_ok(dtype) && mx_format_ok(format), "%s: unknown type or format", who);
-  FL_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && width > 0 && width <= kNormChunks * kMxThreads * 8,
-             "%s: width must be 1 to %d, got %d", who, kNormChunks * kMxThreads * 8, width);
+  FL_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && width > 0 && width <= kMaxNormWidth,
+             "%s: width must be 1 to %d, got %d", who, kMaxNormWidth, width);
   FL_REQUIRE((weight2 == nullptr) == (hidden == nullptr), "%s: weight2 and hidden go together", who);
   FL_REQUIRE(residual == nullptr || weight2 != nullptr, "%s: a residual needs weight2", who);
   FL_REQUIRE(sum_out == nullptr || addend != nullptr, "%s: sum_out needs an addend", who);

@@ -10,6 +10,9 @@
 // a tile of scales is one bulk copy.  Rows of the last tile past the last row hold scale byte 0.
 #pragma once
 
+#include <cstring>
+#include <type_traits>
+
 #include "fl_common.cuh"
 
 namespace fl {
@@ -101,35 +104,45 @@ __device__ __forceinline__ uint32_t mx_join_scales(uint32_t byte) {
   return word | __shfl_xor_sync(0xffffffffu, word, 8);
 }
 
-// Eight consecutive elements as float32: `count` of them exist, the others read as zero.  VEC loads
-// 16 bytes at a time (the caller has checked the alignment of the base and of the row stride).
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int count, float (&v)[8]) {
-  if (VEC && count >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      const uint4 a = ldg128(p), b = ldg128(p + 4);
-      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+// Eight consecutive elements as they lie in memory, so that a load can be under way while others are
+// used.  `count` of them exist (none if it is not positive), the others are zero.  VEC loads 16 bytes at a
+// time (the caller has checked the alignment of the base and of the row stride).
+template <typename T>
+struct Raw8 {
+  static constexpr int kWords = sizeof(T) / 2;  // of 16 bytes
+  uint4 w[kWords];
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T* p, int count) {
+    if (VEC && count >= 8) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(w[k]);
-    } else {
-      const uint4 a = ldg128(p);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+      for (int i = 0; i < kWords; ++i) w[i] = ldg128(reinterpret_cast<const uint4*>(p) + i);
+      return;
+    }
+    T t[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
-          v[2 * k] = bf16_lo(w[k]);
-          v[2 * k + 1] = bf16_hi(w[k]);
-        } else {
-          const float2 f = __half22float2(as_half2(w[k]));
-          v[2 * k] = f.x;
-          v[2 * k + 1] = f.y;
-        }
+    for (int k = 0; k < 8; ++k) t[k] = k < count ? p[k] : T(0.f);
+    memcpy(w, t, sizeof(t));
+  }
+  __device__ __forceinline__ void unpack(float (&v)[8]) const {
+    const uint32_t u[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[kWords - 1].x, w[kWords - 1].y, w[kWords - 1].z,
+                                    w[kWords - 1].w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if constexpr (sizeof(T) == 4) {
+        v[k] = __uint_as_float(u[k]);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        v[k] = k & 1 ? __high2float(as_half2(u[k / 2])) : __low2float(as_half2(u[k / 2]));
+      } else {
+        v[k] = k & 1 ? bf16_hi(u[k / 2]) : bf16_lo(u[k / 2]);
       }
     }
-    return;
   }
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = k < count ? load_as_float<T>(p + k) : 0.f;
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* p, int count, float (&v)[8]) {
+  Raw8<T> raw;
+  raw.template load<VEC>(p, count);
+  raw.unpack(v);
 }
 
 template <typename T>

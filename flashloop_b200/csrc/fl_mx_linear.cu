@@ -179,23 +179,41 @@ __device__ __forceinline__ void emit_rows(const Output& o, int64_t m, int n, con
     for (int j = 0; j < N; ++j)
       if (WHOLE || (live && j < count)) dst[int64_t(j) * o.features] = round_to<T>(v[j]);
   } else {
+    // m is a multiple of N, a divisor of 32, so that the scales of these rows lie sixteen bytes apart
+    static_assert(N % 4 == 0 && 32 % N == 0, "rows of one scale group, four to a word");
     constexpr int kFormat = KIND == kOutFp8 ? FL_MX_FP8 : FL_MX_FP4;
+    const int lane = threadIdx.x & 31;
     const int64_t row_bytes = int64_t(o.w_tiles) * (KIND == kOutFp8 ? kMxStep : kMxStep / 2);
-    uint8_t* codes = static_cast<uint8_t*>(o.data) + m * row_bytes + (KIND == kOutFp8 ? n : n / 2);
+    float q[N];
+    uint32_t mine = 0;  // the scale of row `lane`
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      if (!WHOLE && j >= count) break;  // the same for the warp
-      const float x = live ? v[j] : 0.f;
-      const uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(x) & 0x7fffffffu);
+      q[j] = live && (WHOLE || j < count) ? v[j] : 0.f;
+      const uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(q[j]) & 0x7fffffffu);
       const uint32_t byte = mx_scale_byte<kFormat>(amax);
-      const float q = byte == 255u ? 0.f : x * mx_inverse(byte);
-      if constexpr (KIND == kOutFp8) {
-        codes[j * row_bytes] = uint8_t(cvt_e4m3x2(q, 0.f));
-      } else {
-        const float odd = __shfl_down_sync(0xffffffffu, q, 1);
-        if ((n & 1) == 0) codes[j * row_bytes] = uint8_t(cvt_e2m1x2(q, odd));
+      q[j] = byte == 255u ? 0.f : q[j] * mx_inverse(byte);
+      mine = lane == j ? byte : mine;
+    }
+    if (lane < (WHOLE ? N : min(N, count)))
+      o.scales[mx_scale_offset(m, n / kMxStep, o.w_tiles) + lane * 16 + n / kMxBlock % 4] = uint8_t(mine);
+    if constexpr (KIND == kOutFp8) {
+      // The codes of four rows in a word, then a 4 x 4 transposition of bytes within each four lanes: a lane
+      // has four features of row (lane % 4) and stores them at once.
+      uint8_t* codes = static_cast<uint8_t*>(o.data) + (m + (lane & 3)) * row_bytes + (n & ~3);
+#pragma unroll
+      for (int j = 0; j < N; j += 4) {
+        uint32_t x = __byte_perm(cvt_e4m3x2(q[j], q[j + 1]), cvt_e4m3x2(q[j + 2], q[j + 3]), 0x5410);
+        x = __byte_perm(x, __shfl_xor_sync(0xffffffffu, x, 1), lane & 1 ? 0x3715 : 0x6240);
+        x = __byte_perm(x, __shfl_xor_sync(0xffffffffu, x, 2), lane & 2 ? 0x3276 : 0x5410);
+        if (WHOLE || j + (lane & 3) < count) *reinterpret_cast<uint32_t*>(codes + j * row_bytes) = x;
       }
-      if ((n & 31) == 0) o.scales[mx_scale_offset(m + j, n / kMxStep, o.w_tiles) + n / kMxBlock % 4] = uint8_t(byte);
+    } else {
+      uint8_t* codes = static_cast<uint8_t*>(o.data) + m * row_bytes + n / 2;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float odd = __shfl_down_sync(0xffffffffu, q[j], 1);
+        if ((n & 1) == 0 && (WHOLE || j < count)) codes[j * row_bytes] = uint8_t(cvt_e2m1x2(q[j], odd));
+      }
     }
   }
 }
@@ -239,7 +257,7 @@ struct FewRows {
 // takes is latency, so the copies start before anything else, issued by four warps, and a split sends
 // its sums straight into the shared memory of the CTA that finishes them, which waits for their bytes.
 template <int KIND, int NT, bool DUAL>
-__global__ void __launch_bounds__(kLinThreads)
+__global__ void __launch_bounds__(kLinThreads, 1)
 mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w0,
                  const __grid_constant__ CUtensorMap map_w1, const LinearParams p) {
   using Shape = FewRows<NT, DUAL>;

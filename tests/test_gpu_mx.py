@@ -166,6 +166,9 @@ def test_norm_of_rows_that_are_zero_or_not_finite():
     w = torch.ones(256, device="cuda", dtype=torch.bfloat16)
     y = fl.mx_rmsnorm(x, w, 1e-6)[0].dequantize()
     assert not y[1].any() and torch.isnan(y[2]).all() and torch.isfinite(y[[0, 3]]).all()
+    narrow = fl.mx_rmsnorm(x[:, :40].contiguous(), w[:40], 1e-6)[0]  # row 2 holds the NaN: its padding stays zero
+    byte = ref.scale_bytes(narrow.scales, 4)
+    assert byte[2].tolist() == [255, 255, 0, 0] and not byte[4:].any() and not narrow.codes[:, 40:].any()
 
 
 def _operands(rows, cols, features, x_format, w_format, weights=1):
