@@ -1,4 +1,5 @@
 // Quantisation to the microscaled formats, its inverse, and the RMSNorm that leaves its rows in one.
+#include <algorithm>
 #include <cstring>
 #include <type_traits>
 
@@ -9,35 +10,36 @@ namespace {
 
 constexpr int kMxThreads = 256;
 
-// Sixteen lanes take one step (128 elements) of a row, eight elements each: four lanes share a block,
-// whose largest magnitude takes two shuffles, and the four scale bytes of the step leave as one word.
-// A CTA takes UNROLL * 16 consecutive steps and asks for all of its elements before it uses any.
+// Eight lanes take one step (128 elements) of a row, sixteen elements each: two lanes share a block, and
+// the four scale bytes of the step leave as one word.  A CTA takes UNROLL * 32 consecutive steps and asks for all of its elements before it uses any.
 template <typename T, int FORMAT, bool VEC, int UNROLL>
 __global__ void __launch_bounds__(kMxThreads)
 quantize_kernel(const T* __restrict__ x, uint32_t rows, int cols, int64_t row_stride, uint32_t steps, uint32_t units,
                 uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  const uint32_t first = blockIdx.x * (UNROLL * kMxThreads / 16) + threadIdx.x / 16;
-  const int lane = threadIdx.x & 15;
-  Raw8<T> raw[UNROLL];
+  const uint32_t first = blockIdx.x * (UNROLL * kMxThreads / 8) + threadIdx.x / 8;
+  const int lane = threadIdx.x & 7;
+  __shared__ __align__(16) WarpStage<T, VEC, kMxThreads> stage;
+  Raw16<T> raw[UNROLL];
   uint32_t row[UNROLL];
   int e[UNROLL];
 #pragma unroll
   for (int i = 0; i < UNROLL; ++i) {
-    const uint32_t unit = first + i * (kMxThreads / 16);
+    const uint32_t unit = first + i * (kMxThreads / 8);
     row[i] = unit / steps;
-    e[i] = int(unit - row[i] * steps) * kMxStep + lane * 8;
-    raw[i].template load<VEC>(x + int64_t(row[i]) * row_stride + e[i], unit < units && row[i] < rows ? cols - e[i] : 0);
+    e[i] = int(unit - row[i] * steps) * kMxStep + lane * 16;
+    raw[i].template load<VEC>(x + int64_t(row[i]) * row_stride + e[i], unit < units && row[i] < rows ? cols - e[i] : 0,
+                               stage.mine());
   }
 #pragma unroll
   for (int i = 0; i < UNROLL; ++i) {
-    const uint32_t unit = first + i * (kMxThreads / 16);
-    float v[8];
+    const uint32_t unit = first + i * (kMxThreads / 8);
+    float v[16];
     raw[i].unpack(v);
-    uint32_t out[2];
-    const uint32_t word = mx_join_scales(mx_encode8<FORMAT>(v, out));
+    uint32_t out[4];
+    const uint32_t word = mx_join_scales(mx_encode16<FORMAT>(v, out));
     if (unit >= units) continue;
     if (row[i] < rows) {
-      store_codes<FORMAT>(codes + int64_t(unit) * (FORMAT == FL_MX_FP8 ? kMxStep : kMxStep / 2), lane * 8, out);
+      store_codes<FORMAT>(codes + int64_t(unit) * (FORMAT == FL_MX_FP8 ? kMxStep : kMxStep / 2), lane * 16, out);
     }
     // steps past the last row belong to the last scale tile: their values are zero, and so is the word
     if (lane == 0)
@@ -45,63 +47,63 @@ quantize_kernel(const T* __restrict__ x, uint32_t rows, int cols, int64_t row_st
   }
 }
 
-// Eight elements of a row per thread and round.
-template <typename T, int FORMAT, int UNROLL>
+// Sixteen elements of a row per thread and round.
+template <typename T, int FORMAT, bool VEC, int UNROLL>
 __global__ void __launch_bounds__(kMxThreads)
 dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int cols, uint32_t steps,
                   uint32_t units, T* __restrict__ out) {
-  const uint32_t first = blockIdx.x * (UNROLL * kMxThreads / 16) + threadIdx.x / 16;
-  const int lane = threadIdx.x & 15;
-  uint2 word[UNROLL] = {};
+  const uint32_t first = blockIdx.x * (UNROLL * kMxThreads / 8) + threadIdx.x / 8;
+  const int lane = threadIdx.x & 7;
+  __shared__ __align__(16) WarpStage<T, VEC, kMxThreads> stage;
+  uint4 word[UNROLL] = {};
   uint32_t byte[UNROLL] = {};
   uint32_t row[UNROLL];
   int e[UNROLL];
 #pragma unroll
   for (int i = 0; i < UNROLL; ++i) {
-    const uint32_t unit = first + i * (kMxThreads / 16);
+    const uint32_t unit = first + i * (kMxThreads / 8);
     row[i] = unit / steps;
     const uint32_t step = unit - row[i] * steps;
-    e[i] = unit < units ? int(step) * kMxStep + lane * 8 : cols;
+    e[i] = unit < units ? int(step) * kMxStep + lane * 16 : cols;
     if (e[i] < cols) {
       const uint8_t* src = codes + int64_t(unit) * (FORMAT == FL_MX_FP8 ? kMxStep : kMxStep / 2);
       if (FORMAT == FL_MX_FP8) {
-        word[i] = ldg64(src + lane * 8);
+        word[i] = ldg128(src + lane * 16);
       } else {
-        word[i].x = __ldg(reinterpret_cast<const uint32_t*>(src + lane * 4));
+        const uint2 half = ldg64(src + lane * 8);
+        word[i].x = half.x;
+        word[i].y = half.y;
       }
-      byte[i] = __ldg(scales + mx_scale_offset(row[i], step, steps) + lane / 4);
+      byte[i] = __ldg(scales + mx_scale_offset(row[i], step, steps) + lane / 2);
     }
   }
 #pragma unroll
   for (int i = 0; i < UNROLL; ++i) {
-    if (e[i] >= cols) continue;
+    if (VEC && e[i] >= cols) continue;
     const float scale = mx_scale_value(byte[i]);
-    float v[8];
+    const uint32_t w[4] = {word[i].x, word[i].y, word[i].z, word[i].w};
+    float v[16];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 8; ++k) {
       uint32_t h;
       if (FORMAT == FL_MX_FP8) {
-        const uint16_t pair = uint16_t((k < 2 ? word[i].x : word[i].y) >> (16 * (k & 1)));
+        const uint16_t pair = uint16_t(w[k / 2] >> (16 * (k & 1)));
         asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(pair));
       } else {
-        asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"((word[i].x >> (8 * k)) & 255u));
+        asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"((w[k / 4] >> (8 * (k & 3))) & 255u));
       }
       const float2 f = __half22float2(as_half2(h));
       v[2 * k] = f.x * scale;
       v[2 * k + 1] = f.y * scale;
     }
-    T* dst = out + int64_t(row[i]) * cols + e[i];
-    if (cols % 8 == 0) {
-      store8<T, true>(dst, cols - e[i], v);
-    } else {
-      store8<T, false>(dst, cols - e[i], v);
-    }
+    store16<T, VEC>(out + int64_t(row[i]) * cols + e[i], cols - e[i], v, stage.mine());
   }
 }
 
-// Rows up to 8192 wide: eight warps of four chunks of eight elements per thread, four of eight chunks.
+// Rows up to 8192 wide: eight warps of two chunks of sixteen elements per thread.
 constexpr int kMaxNormWidth = 8192;
 constexpr int64_t kManyRows = 148 * 8;
+constexpr int kNormSmThreads = 768, kNormSmThreads2 = 512;  // threads of the persistent CTAs per SM, without and with weight2
 
 template <typename T>
 struct MxNormParams {
@@ -120,18 +122,18 @@ struct MxNormParams {
   uint8_t* scales;
 };
 
-// Sum over the warps of a row; every thread gets it.
+// Sum over the warps of a row; every thread gets it.  `part` alternates between calls, so that one
+// barrier is enough.
 template <int WARPS>
-__device__ __forceinline__ float row_sum(float v, float* s_part) {
+__device__ __forceinline__ float row_sum(float v, float* part) {
   v = warp_sum(v);
   if (WARPS == 1) return v;
   const int warp = threadIdx.x >> 5, first = warp / WARPS * WARPS;
-  __syncthreads();  // s_part may still be read from the previous sum
-  if ((threadIdx.x & 31) == 0) s_part[warp] = v;
+  if ((threadIdx.x & 31) == 0) part[warp] = v;
   __syncthreads();
   float total = 0.f;
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) total += s_part[first + w];
+  for (int w = 0; w < WARPS; ++w) total += part[first + w];
   return total;
 }
 
@@ -148,96 +150,125 @@ __device__ __forceinline__ float inverse_root(float sum, int width, float eps) {
 // those of n; with it hidden = round([residual +] n) and the codes are those of weight2 * hidden *
 // rsqrt(mean(hidden^2) + eps2).  Everything between two stored tensors stays in float32.
 //
-// WARPS warps share a row and hold it in registers, CHUNKS times eight elements per thread; what the
-// row needs from memory is requested before the first sum.  Many rows take few warps each, with no
-// barrier but that of the warp: bound by memory (MEASURED).  Few rows take eight: bound by latency.
-template <typename T, int FORMAT, bool VEC, int WARPS, int CHUNKS>
-__global__ void __launch_bounds__(kMxThreads) norm_mx_kernel(const MxNormParams<T> p) {
-  constexpr int kRowThreads = WARPS * 32, kRows = kMxThreads / kRowThreads;
-  __shared__ float s_part[kMxThreads / 32];
-  const int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / kRowThreads;
-  const int thread = threadIdx.x % kRowThreads;
-  const bool live = row < p.rows;
-  const int64_t base = row * p.width;
-  Raw8<T> raw_x[CHUNKS], raw_a[CHUNKS], raw_r[CHUNKS];
+// WARPS warps share a row and hold it in registers, CHUNKS times sixteen elements per thread.  Many
+// rows: CTAs of as few warps as hold a row, each taking row after row and asking for the next one before it works on
+// the present one; bound by memory (32768 x 2048 bfloat16 with residual and second norm: 80 us, 5.9 TB/s of the copy rate of
+// 6.5).  Few rows: a CTA each; bound by latency.
+template <int WARPS>
+constexpr int kNormThreads = WARPS < 4 ? 128 : WARPS * 32;
+
+template <typename T, int CHUNKS, bool SECOND>
+struct NormRow {
+  Raw16<T> x[CHUNKS], a[CHUNKS], r[SECOND ? CHUNKS : 1];
+  template <bool VEC, int ROW_THREADS>
+  __device__ __forceinline__ void load(const MxNormParams<T>& p, int64_t row, int thread, T* stage) {
+    const int64_t base = row * p.width;
 #pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
-    const int e = (c * kRowThreads + thread) * 8, n = live ? p.width - e : 0;
-    raw_x[c].template load<VEC>(p.x + base + e, n);
-    if (p.addend) raw_a[c].template load<VEC>(p.addend + base + e, n);
-    if (p.residual) raw_r[c].template load<VEC>(p.residual + base + e, n);
-  }
-  float v[CHUNKS][8];
-  float sq = 0.f;
-#pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
-    raw_x[c].unpack(v[c]);
-    if (p.addend) {
-      const int e = (c * kRowThreads + thread) * 8, n = live ? p.width - e : 0;
-      float a[8];
-      raw_a[c].unpack(a);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[c][k] += a[k];
-      store8<T, VEC>(p.sum_out && n > 0 ? p.sum_out + base + e : nullptr, n, v[c]);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) sq = fmaf(v[c][k], v[c][k], sq);
-  }
-  float inv = inverse_root(row_sum<WARPS>(sq, s_part), p.width, p.eps);
-  sq = 0.f;
-#pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
-    const int e = (c * kRowThreads + thread) * 8, n = live ? p.width - e : 0;
-    float w[8];
-    load8<T, VEC>(p.weight + e, p.width - e, w);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[c][k] = w[k] * (v[c][k] * inv);
-    if (p.weight2) {
-      if (p.residual) {
-        float r[8];
-        raw_r[c].unpack(r);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[c][k] += r[k];
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int e = (c * ROW_THREADS + thread) * 16, n = row < p.rows ? p.width - e : 0;
+      x[c].template load<VEC>(p.x + base + e, n, stage);
+      if (p.addend) a[c].template load<VEC>(p.addend + base + e, n, stage);
+      if constexpr (SECOND) {
+        if (p.residual) r[c].template load<VEC>(p.residual + base + e, n, stage);
       }
-      store8<T, VEC>(n > 0 ? p.hidden + base + e : nullptr, n, v[c]);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sq = fmaf(v[c][k], v[c][k], sq);
     }
   }
-  if (p.weight2) inv = inverse_root(row_sum<WARPS>(sq, s_part), p.width, p.eps2);
-  uint8_t* codes = p.codes + row * p.steps * (FORMAT == FL_MX_FP8 ? kMxStep : kMxStep / 2);
+};
+
+// SECOND: weight2 is given.
+template <typename T, int FORMAT, bool VEC, bool SECOND, int WARPS, int CHUNKS>
+__global__ void __launch_bounds__(kNormThreads<WARPS>) norm_mx_kernel(const MxNormParams<T> p) {
+  constexpr int kThreads = kNormThreads<WARPS>, kRowThreads = WARPS * 32, kRows = kThreads / kRowThreads;
+  __shared__ float s_part[2][kThreads / 32];
+  __shared__ __align__(16) WarpStage<T, VEC, kThreads> stage;
+  const int thread = threadIdx.x % kRowThreads;
+  const int64_t stride = int64_t(gridDim.x) * kRows;
   const bool one_group = p.rows <= 32;  // a row's word is then the only one of its sixteen bytes
+  int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / kRowThreads;
+  NormRow<T, CHUNKS, SECOND> next;
+  next.template load<VEC, kRowThreads>(p, row, thread, stage.mine());
+  float w[CHUNKS][16], w2[SECOND ? CHUNKS : 1][16];
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-    const int e = (c * kRowThreads + thread) * 8;
-    const uint32_t step = uint32_t(e) / kMxStep;
-    if (c * kRowThreads * 8 >= p.width) continue;  // the same for the whole CTA
-    if (p.weight2) {
-      float w[8];
-      load8<T, VEC>(p.weight2 + e, p.width - e, w);
+    const int e = (c * kRowThreads + thread) * 16;
+    load16<T, VEC>(p.weight + e, p.width - e, w[c], stage.mine());
+    if constexpr (SECOND) load16<T, VEC>(p.weight2 + e, p.width - e, w2[c], stage.mine());
+  }
+  // the same number of rounds for all threads of the CTA, which meet at barriers
+  for (int64_t first = int64_t(blockIdx.x) * kRows; first < p.rows; first += stride, row += stride) {
+    const bool live = row < p.rows;
+    const int64_t base = row * p.width;
+    NormRow<T, CHUNKS, SECOND> now = next;
+    if (first + stride < p.rows) next.template load<VEC, kRowThreads>(p, row + stride, thread, stage.mine());
+    float v[CHUNKS][16];
+    float sq = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[c][k] = w[k] * (v[c][k] * inv);
-    }
-    if (e >= p.width) {  // padding is zero also where the row is not finite
+    for (int c = 0; c < CHUNKS; ++c) {
+      now.x[c].unpack(v[c]);
+      if (p.addend) {
+        const int e = (c * kRowThreads + thread) * 16, n = live ? p.width - e : 0;
+        float a[16];
+        now.a[c].unpack(a);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[c][k] = 0.f;
+        for (int k = 0; k < 16; ++k) v[c][k] += a[k];
+        store16<T, VEC>(p.sum_out + base + e, p.sum_out ? n : 0, v[c], stage.mine());
+      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k) sq = fmaf(v[c][k], v[c][k], sq);
     }
-    uint32_t out[2];
-    const uint32_t word = mx_join_scales(mx_encode8<FORMAT>(v[c], out));
-    if (live && step < p.steps) {
-      store_codes<FORMAT>(codes, e, out);
-      if ((threadIdx.x & 15) == 0) {
-        uint8_t* at = p.scales + mx_scale_offset(row, step, p.steps);
-        if (one_group) {
-          *reinterpret_cast<uint4*>(at) = make_uint4(word, 0u, 0u, 0u);
-        } else {
-          *reinterpret_cast<uint32_t*>(at) = word;
+    float inv = inverse_root(row_sum<WARPS>(sq, s_part[0]), p.width, p.eps);
+    sq = 0.f;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      float r[16] = {};
+      if constexpr (SECOND) {
+        if (p.residual) now.r[c].unpack(r);
+      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[c][k] = fmaf(w[c][k], v[c][k] * inv, r[k]);
+      if constexpr (SECOND) {
+        const int e = (c * kRowThreads + thread) * 16, n = live ? p.width - e : 0;
+        store16<T, VEC>(p.hidden + base + e, n, v[c], stage.mine());
+#pragma unroll
+        for (int k = 0; k < 16; ++k) sq = fmaf(v[c][k], v[c][k], sq);
+      }
+    }
+    // one barrier per round orders the reads of s_part[0] before its next writes, and the second sum's does s_part[1]
+    if constexpr (SECOND) {
+      inv = inverse_root(row_sum<WARPS>(sq, s_part[1]), p.width, p.eps2);
+    } else if (WARPS > 1) {
+      __syncthreads();
+    }
+    uint8_t* codes = p.codes + row * p.steps * (FORMAT == FL_MX_FP8 ? kMxStep : kMxStep / 2);
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int e = (c * kRowThreads + thread) * 16;
+      const uint32_t step = uint32_t(e) / kMxStep;
+      if constexpr (SECOND) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[c][k] = w2[c][k] * (v[c][k] * inv);
+      }
+      if (e >= p.width) {  // padding is zero also where the row is not finite
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[c][k] = 0.f;
+      }
+      uint32_t out[4];
+      const uint32_t word = mx_join_scales(mx_encode16<FORMAT>(v[c], out));
+      if (live && step < p.steps) {
+        store_codes<FORMAT>(codes, e, out);
+        if ((threadIdx.x & 7) == 0) {
+          uint8_t* at = p.scales + mx_scale_offset(row, step, p.steps);
+          if (one_group) {
+            *reinterpret_cast<uint4*>(at) = make_uint4(word, 0u, 0u, 0u);
+          } else {
+            *reinterpret_cast<uint32_t*>(at) = word;
+          }
         }
       }
     }
   }
   // rows of the last scale tile past the last row, shared out over all threads
-  const uint32_t threads = gridDim.x * kMxThreads, mine = blockIdx.x * kMxThreads + threadIdx.x;
+  const uint32_t threads = gridDim.x * kThreads, mine = blockIdx.x * kThreads + threadIdx.x;
   if (one_group) {
     const uint32_t empty = 32u - uint32_t(p.rows);  // sixteen-byte groups of a step that hold no row
     for (uint32_t i = mine; i < empty * p.steps; i += threads)
@@ -257,9 +288,9 @@ void launch_quantize(const T* x, int64_t rows, int32_t cols, int64_t stride, uin
                      void* scales, cudaStream_t stream) {
   uint8_t* c = static_cast<uint8_t*>(codes);
   uint8_t* s = static_cast<uint8_t*>(scales);
-  constexpr int kUnits = kMxThreads / 16;
+  constexpr int kUnits = kMxThreads / 8;
   if (units >= kUnrollUnits) {
-    quantize_kernel<T, FORMAT, VEC, 4><<<(units + 4 * kUnits - 1) / (4 * kUnits), kMxThreads, 0, stream>>>(
+    quantize_kernel<T, FORMAT, VEC, 2><<<(units + 2 * kUnits - 1) / (2 * kUnits), kMxThreads, 0, stream>>>(
         x, uint32_t(rows), cols, stride, steps, units, c, s);
   } else {
     quantize_kernel<T, FORMAT, VEC, 1><<<(units + kUnits - 1) / kUnits, kMxThreads, 0, stream>>>(
@@ -288,16 +319,15 @@ int launch_dequantize(const void* codes, const void* scales, int64_t rows, int32
                       cudaStream_t stream) {
   const int64_t steps = mx_steps(cols), units = rows * steps;
   FL_REQUIRE(units < (int64_t(1) << 31), "fl_mx_dequantize: too many elements");
-  constexpr int kUnits = kMxThreads / 16;
+  constexpr int kUnits = kMxThreads / 8;
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   const uint8_t* s = static_cast<const uint8_t*>(scales);
-  if (units >= kUnrollUnits) {
-    dequantize_kernel<T, FORMAT, 4><<<unsigned((units + 4 * kUnits - 1) / (4 * kUnits)), kMxThreads, 0, stream>>>(
-        c, s, cols, uint32_t(steps), uint32_t(units), static_cast<T*>(out));
-  } else {
-    dequantize_kernel<T, FORMAT, 1><<<unsigned((units + kUnits - 1) / kUnits), kMxThreads, 0, stream>>>(
-        c, s, cols, uint32_t(steps), uint32_t(units), static_cast<T*>(out));
-  }
+  const bool many = units >= kUnrollUnits, vec = cols * sizeof(T) % 16 == 0;
+  auto kernel = many ? (vec ? dequantize_kernel<T, FORMAT, true, 4> : dequantize_kernel<T, FORMAT, false, 4>)
+                     : (vec ? dequantize_kernel<T, FORMAT, true, 1> : dequantize_kernel<T, FORMAT, false, 1>);
+  const int64_t each = many ? 4 * kUnits : kUnits;
+  kernel<<<unsigned((units + each - 1) / each), kMxThreads, 0, stream>>>(c, s, cols, uint32_t(steps), uint32_t(units),
+                                                                        static_cast<T*>(out));
   FL_CHECK_LAUNCH("fl_mx_dequantize");
   return FL_OK;
 }
@@ -310,23 +340,22 @@ struct NormArgs {
   void *sum_out, *hidden, *codes, *scales;
 };
 
-template <typename T, int FORMAT, bool VEC, int WARPS, int CHUNKS>
+template <typename T, int FORMAT, bool VEC, bool SECOND, int WARPS, int CHUNKS>
 void launch_norm_shape(const MxNormParams<T>& p, cudaStream_t stream) {
-  constexpr int kRows = kMxThreads / 32 / WARPS;
-  norm_mx_kernel<T, FORMAT, VEC, WARPS, CHUNKS><<<unsigned((p.rows + kRows - 1) / kRows), kMxThreads, 0, stream>>>(p);
+  constexpr int kThreads = kNormThreads<WARPS>, kRows = kThreads / 32 / WARPS;
+  const int64_t ctas = std::min<int64_t>((p.rows + kRows - 1) / kRows, 148 * ((SECOND ? kNormSmThreads2 : kNormSmThreads) / kThreads));
+  norm_mx_kernel<T, FORMAT, VEC, SECOND, WARPS, CHUNKS><<<unsigned(ctas), kThreads, 0, stream>>>(p);
 }
 
-// Warps to a row: as few as hold it once there are rows enough to fill the SMs, otherwise all eight of a CTA.
-template <typename T, int FORMAT, bool VEC>
+// Warps to a row: as few as hold it once there are rows enough to fill the SMs, otherwise eight.
+template <typename T, int FORMAT, bool VEC, bool SECOND>
 void launch_norm_rows(const MxNormParams<T>& p, cudaStream_t stream) {
   const bool many = p.rows >= kManyRows;
-  if (many && p.width <= 512) return launch_norm_shape<T, FORMAT, VEC, 1, 2>(p, stream);
-  if (many && p.width <= 1024) return launch_norm_shape<T, FORMAT, VEC, 1, 4>(p, stream);
-  if (many && p.width <= 2048) return launch_norm_shape<T, FORMAT, VEC, 2, 4>(p, stream);
-  if (many && p.width <= 4096) return launch_norm_shape<T, FORMAT, VEC, 4, 4>(p, stream);
-  if (p.width <= 2048) return launch_norm_shape<T, FORMAT, VEC, 8, 1>(p, stream);
-  if (p.width <= 4096) return launch_norm_shape<T, FORMAT, VEC, 8, 2>(p, stream);
-  return launch_norm_shape<T, FORMAT, VEC, 8, 4>(p, stream);
+  if (many && p.width <= 512) return launch_norm_shape<T, FORMAT, VEC, SECOND, 1, 1>(p, stream);
+  if (many && p.width <= 1024) return launch_norm_shape<T, FORMAT, VEC, SECOND, 2, 1>(p, stream);
+  if (p.width <= 2048) return launch_norm_shape<T, FORMAT, VEC, SECOND, 4, 1>(p, stream);
+  if (p.width <= 4096) return launch_norm_shape<T, FORMAT, VEC, SECOND, 8, 1>(p, stream);
+  return launch_norm_shape<T, FORMAT, VEC, SECOND, 8, 2>(p, stream);
 }
 
 template <typename T, int FORMAT>
@@ -350,9 +379,9 @@ int launch_norm(const NormArgs& a, cudaStream_t stream) {
                    aligned16(a.weight2) && aligned16(a.sum_out) && aligned16(a.hidden) &&
                    a.width * sizeof(T) % 16 == 0;
   if (vec) {
-    launch_norm_rows<T, FORMAT, true>(p, stream);
+    a.weight2 ? launch_norm_rows<T, FORMAT, true, true>(p, stream) : launch_norm_rows<T, FORMAT, true, false>(p, stream);
   } else {
-    launch_norm_rows<T, FORMAT, false>(p, stream);
+    a.weight2 ? launch_norm_rows<T, FORMAT, false, true>(p, stream) : launch_norm_rows<T, FORMAT, false, false>(p, stream);
   }
   FL_CHECK_LAUNCH("fl_rmsnorm_mx");
   return FL_OK;

@@ -74,74 +74,115 @@ __device__ __forceinline__ uint32_t cvt_e2m1x2(float lo, float hi) {
   return r;
 }
 
-// Eight values of one block, held by one of the four lanes that share it (lanes 4i .. 4i + 3).
-// Returns the block's scale byte and writes the codes: e4m3 into codes[0..1], e2m1 into codes[0].
+// Sixteen values of one block, held by one of the two lanes that share it (lanes 2i and 2i + 1).
+// Returns the block's scale byte and writes the codes: e4m3 into codes[0..3], e2m1 into codes[0..1].
 template <int FORMAT>
-__device__ __forceinline__ uint32_t mx_encode8(const float (&v)[8], uint32_t (&codes)[2]) {
-  uint32_t amax = 0;
+__device__ __forceinline__ uint32_t mx_encode16(const float (&v)[16], uint32_t (&codes)[4]) {
+  float top = fabsf(v[0]);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) amax = max(amax, __float_as_uint(v[k]) & 0x7fffffffu);
+  for (int k = 1; k < 15; k += 2)  // the largest of three in one instruction, a NaN if there is one
+    asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(fabsf(v[k])), "f"(fabsf(v[k + 1])));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(v[15])));
+  uint32_t amax = __float_as_uint(top) & 0x7fffffffu;
   amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
   const uint32_t byte = mx_scale_byte<FORMAT>(amax);
   const float inv = mx_inverse(byte);
-  if (byte == 255u) {
-    codes[0] = codes[1] = 0u;
-  } else if (FORMAT == FL_MX_FP8) {
-    codes[0] = cvt_e4m3x2(v[0] * inv, v[1] * inv) | cvt_e4m3x2(v[2] * inv, v[3] * inv) << 16;
-    codes[1] = cvt_e4m3x2(v[4] * inv, v[5] * inv) | cvt_e4m3x2(v[6] * inv, v[7] * inv) << 16;
-  } else {
-    codes[0] = cvt_e2m1x2(v[0] * inv, v[1] * inv) | cvt_e2m1x2(v[2] * inv, v[3] * inv) << 8 |
-               cvt_e2m1x2(v[4] * inv, v[5] * inv) << 16 | cvt_e2m1x2(v[6] * inv, v[7] * inv) << 24;
-    codes[1] = 0u;
+  const uint32_t keep = byte == 255u ? 0u : 0xffffffffu;  // a block that is not finite has codes 0
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = v[4 * i] * inv, b = v[4 * i + 1] * inv, c = v[4 * i + 2] * inv, d = v[4 * i + 3] * inv;
+    if (FORMAT == FL_MX_FP8) {
+      codes[i] = __byte_perm(cvt_e4m3x2(a, b), cvt_e4m3x2(c, d), 0x5410) & keep;
+    } else {
+      const uint32_t w = __byte_perm(cvt_e2m1x2(a, b), cvt_e2m1x2(c, d), 0x3340) & keep;
+      if (i % 2 == 0) {
+        codes[i / 2] = w;
+      } else {
+        codes[i / 2] |= w << 16;
+      }
+    }
   }
   return byte;
 }
-// The four scale bytes of a step from the sixteen lanes that hold it, in every one of them.
+// The four scale bytes of a step from the eight lanes that hold it, in every one of them.
 __device__ __forceinline__ uint32_t mx_join_scales(uint32_t byte) {
-  uint32_t word = byte << (8 * ((threadIdx.x >> 2) & 3));
-  word |= __shfl_xor_sync(0xffffffffu, word, 4);
-  return word | __shfl_xor_sync(0xffffffffu, word, 8);
+  uint32_t word = byte << (8 * ((threadIdx.x >> 1) & 3));
+  word |= __shfl_xor_sync(0xffffffffu, word, 2);
+  return word | __shfl_xor_sync(0xffffffffu, word, 4);
 }
 
-// Eight consecutive elements as they lie in memory, so that a load can be under way while others are
-// used.  `count` of them exist (none if it is not positive), the others are zero.  VEC loads 16 bytes at a
-// time (the caller has checked the alignment of the base and of the row stride).
+// Sixteen consecutive elements as they lie in memory, so that a load can be under way while others are
+// used.  `count` of them exist (none if it is not positive), the others are zero.
+// VEC: loads of 16 bytes (the caller has checked the alignment of the base and of the row stride), of 32
+// where the address allows.  Otherwise the warp, whose groups of eight lanes each hold 128 consecutive
+// elements, loads them lane by lane and passes them on through 512 elements of shared memory, `stage`; all of its
+// lanes make the call.
 template <typename T>
-struct Raw8 {
-  static constexpr int kWords = sizeof(T) / 2;  // of 16 bytes
-  uint4 w[kWords];
+struct Raw16 {
+  static constexpr int kWords = 4 * sizeof(T);  // of four bytes
+  uint32_t w[kWords];
   template <bool VEC>
-  __device__ __forceinline__ void load(const T* p, int count) {
-    if (VEC && count >= 8) {
+  __device__ __forceinline__ void load(const T* p, int count, T* stage) {
+    if constexpr (VEC) {
+      if (count >= 16) {
+        if ((reinterpret_cast<uintptr_t>(p) & 31) == 0) {
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) w[i] = ldg128(reinterpret_cast<const uint4*>(p) + i);
-      return;
-    }
-    T t[8];
+          for (int i = 0; i < kWords; i += 8)
+            asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]),
+                  "=r"(w[i + 6]), "=r"(w[i + 7])
+                : "l"(reinterpret_cast<const uint32_t*>(p) + i));
+        } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) t[k] = k < count ? p[k] : T(0.f);
-    memcpy(w, t, sizeof(t));
-  }
-  __device__ __forceinline__ void unpack(float (&v)[8]) const {
-    const uint32_t u[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[kWords - 1].x, w[kWords - 1].y, w[kWords - 1].z,
-                                    w[kWords - 1].w};
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if constexpr (sizeof(T) == 4) {
-        v[k] = __uint_as_float(u[k]);
-      } else if constexpr (std::is_same<T, __half>::value) {
-        v[k] = k & 1 ? __high2float(as_half2(u[k / 2])) : __low2float(as_half2(u[k / 2]));
+          for (int i = 0; i < kWords; i += 4) {
+            const uint4 q = ldg128(reinterpret_cast<const uint32_t*>(p) + i);
+            w[i] = q.x, w[i + 1] = q.y, w[i + 2] = q.z, w[i + 3] = q.w;
+          }
+        }
       } else {
-        v[k] = k & 1 ? bf16_hi(u[k / 2]) : bf16_lo(u[k / 2]);
+        T t[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) t[k] = k < count ? p[k] : T(0.f);
+        memcpy(w, t, sizeof(t));
+      }
+    } else {
+      const int lane = threadIdx.x & 31;
+      T t[16];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const T* base = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(p), g * 8));
+        const int total = __shfl_sync(0xffffffffu, count, g * 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[4 * g + i] = lane + 32 * i < total ? base[lane + 32 * i] : T(0.f);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) stage[lane + 32 * i] = t[i];
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 q = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(stage) + lane * kWords + i);
+        w[i] = q.x, w[i + 1] = q.y, w[i + 2] = q.z, w[i + 3] = q.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void unpack(float (&v)[16]) const {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      if constexpr (sizeof(T) == 4) {
+        v[k] = __uint_as_float(w[k]);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        v[k] = k & 1 ? __high2float(as_half2(w[k / 2])) : __low2float(as_half2(w[k / 2]));
+      } else {
+        v[k] = k & 1 ? bf16_hi(w[k / 2]) : bf16_lo(w[k / 2]);
       }
     }
   }
 };
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int count, float (&v)[8]) {
-  Raw8<T> raw;
-  raw.template load<VEC>(p, count);
+__device__ __forceinline__ void load16(const T* p, int count, float (&v)[16], T* stage) {
+  Raw16<T> raw;
+  raw.template load<VEC>(p, count, stage);
   raw.unpack(v);
 }
 
@@ -154,35 +195,82 @@ __device__ __forceinline__ __half round_to<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ float round_to<float>(float v) { return v; }
 
-// Eight values rounded to T, stored; `v` keeps what was stored.
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, int count, float (&v)[8]) {
-  T t[8];
+// Sixteen values rounded to T.
+template <typename T>
+__device__ __forceinline__ Raw16<T> pack16(const float (&v)[16]) {
+  Raw16<T> raw;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    t[k] = round_to<T>(v[k]);
-    v[k] = load_as_float<T>(&t[k]);
+  for (int i = 0; i < Raw16<T>::kWords; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      raw.w[i] = __float_as_uint(v[i]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      raw.w[i] = as_u32(__floats2half2_rn(v[2 * i], v[2 * i + 1]));
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      memcpy(&raw.w[i], &h, 4);
+    }
   }
-  if (p == nullptr) return;
-  if (VEC && count >= 8) {
-    uint4 w[sizeof(T) / 2];
-    memcpy(w, t, sizeof(t));
-#pragma unroll
-    for (int k = 0; k < int(sizeof(T) / 2); ++k) reinterpret_cast<uint4*>(p)[k] = w[k];
-    return;
-  }
-#pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (k < count) p[k] = t[k];
+  return raw;
 }
 
-// Codes of eight elements starting at element `e` of a row (e a multiple of 8).
-template <int FORMAT>
-__device__ __forceinline__ void store_codes(uint8_t* row_codes, int64_t e, const uint32_t (&codes)[2]) {
-  if (FORMAT == FL_MX_FP8) {
-    *reinterpret_cast<uint2*>(row_codes + e) = make_uint2(codes[0], codes[1]);
+// The first `count` of sixteen values (none if it is not positive) rounded to T and stored; `v` becomes what
+// they are rounded to.  VEC, `stage` and the call by whole warps as for the load.
+template <typename T, bool VEC>
+__device__ __forceinline__ void store16(T* p, int count, float (&v)[16], T* stage) {
+  const Raw16<T> raw = pack16<T>(v);
+  raw.unpack(v);
+  const uint32_t* w = raw.w;
+  if constexpr (VEC) {
+    uint32_t* q = reinterpret_cast<uint32_t*>(p);
+    if (count >= 16 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+#pragma unroll
+      for (int i = 0; i < Raw16<T>::kWords; i += 8)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                     ::"l"(q + i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]),
+                       "r"(w[i + 6]), "r"(w[i + 7]) : "memory");
+    } else if (count >= 16) {
+#pragma unroll
+      for (int i = 0; i < Raw16<T>::kWords; i += 4)
+        *reinterpret_cast<uint4*>(q + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    } else {
+      T t[16];
+      memcpy(t, w, sizeof(t));
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (k < count) p[k] = t[k];
+    }
   } else {
-    *reinterpret_cast<uint32_t*>(row_codes + e / 2) = codes[0];
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < Raw16<T>::kWords; i += 4)
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(stage) + lane * Raw16<T>::kWords + i) =
+          make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      T* base = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(p), g * 8));
+      const int total = __shfl_sync(0xffffffffu, count, g * 8);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (lane + 32 * i < total) base[lane + 32 * i] = stage[g * 128 + lane + 32 * i];
+    }
+  }
+}
+// Shared memory of the warps for loads and stores without VEC.
+template <typename T, bool VEC, int THREADS>
+struct WarpStage {
+  T data[THREADS / 32][VEC ? 16 : 512];
+  __device__ __forceinline__ T* mine() { return data[threadIdx.x >> 5]; }
+};
+
+// Codes of sixteen elements starting at element `e` of a row (e a multiple of 16).
+template <int FORMAT>
+__device__ __forceinline__ void store_codes(uint8_t* row_codes, int64_t e, const uint32_t (&codes)[4]) {
+  if (FORMAT == FL_MX_FP8) {
+    *reinterpret_cast<uint4*>(row_codes + e) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+  } else {
+    *reinterpret_cast<uint2*>(row_codes + e / 2) = make_uint2(codes[0], codes[1]);
   }
 }
 
