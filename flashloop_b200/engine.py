@@ -24,10 +24,11 @@ from .cache import CrossLoopKVCache, CrossLoopKVLayer, CrossLoopKVLayerBuilder
 from .compaction import RetainedTokens, hidden_delta_score, retain_tokens
 from .config import FlashLoopConfig, validate_ouro_model
 from .selection import decode_budget
-from .prefill import PrefillReceipt, apply_rope, dense_prefill_loop, sparse_prefill_loop
+from .mx import mx_linear, mx_linear_swiglu, mx_rmsnorm
+from .prefill import PrefillReceipt, apply_rope, dense_prefill_loop, norm_eps, sparse_prefill_loop
 from . import step_ops
 from .tensor_parallel import PartialSum, PeerAllReduce
-from .weights import fused_mlp, project_qkv, project_value, repack_projection_weights
+from .weights import fused_mlp, project_qkv, project_value, quantize_projection_weights, repack_projection_weights
 
 
 @dataclass(frozen=True)
@@ -66,7 +67,8 @@ class FlashLoopEngine:
     def __init__(self, model: torch.nn.Module, *, config: FlashLoopConfig | None = None,
                  validate_model: bool = True, max_new_tokens: int = 512, use_cuda_graph: bool = False,
                  reference_loop4_scores: bool = True, fuse_decode_ops: bool = True, tp_group=None,
-                 tp_allreduce: str = "peer", tp_wait_limit: int = 0, stream_projections: bool = True) -> None:
+                 tp_allreduce: str = "peer", tp_wait_limit: int = 0, stream_projections: bool = True,
+                 projection_format: str | None = None) -> None:
         if validate_model:
             validate_ouro_model(model)
         elif int(getattr(model.config, "total_ut_steps", 0)) != 4:
@@ -98,6 +100,20 @@ class FlashLoopEngine:
         # the projections of a decode step of at most 16 sequences through this library's weight-
         # streaming kernel (step_ops.linear) instead of the framework's GEMM
         self.stream_projections = bool(stream_projections)
+        # "mxfp4" or "mxfp8": the projection weights of all layers are quantised in place of the bfloat16
+        # ones (which are released), and prefill and decode run on microscaled operands: the norms and the
+        # gated activation leave their rows in mxfp8, the products run on the block-scaled tensor cores
+        # (see mx.py).  The embedding, the norms, attention and lm_head stay as they are.
+        self.projection_format = projection_format
+        if projection_format is not None:
+            if tp_group is not None:
+                raise ValueError("projection_format does not combine with tensor parallelism")
+            if not self.config.fuse_projection_weights or not self.fuse_decode_ops:
+                raise ValueError("projection_format needs fused projection weights and decode ops "
+                                 "(fuse_projection_weights, fuse_decode_ops) and an Ouro-style block")
+            quantize_projection_weights(self.layers, projection_format)
+        elif any(getattr(layer.self_attn, "_flashloop_mx_qkv", None) is not None for layer in self.layers):
+            raise ValueError("the projections of this model are microscaled: pass their projection_format")
         self._reuse = self.config.reuse_selected_probabilities and self.config.enable_sparse_decode
         self._state: EngineState | None = None
         self._graph = None
@@ -214,12 +230,7 @@ class FlashLoopEngine:
 
     # ------------------------------------------------------------------ decode
 
-    @staticmethod
-    def _norm_eps(norm) -> float | None:
-        for name in ("eps", "variance_epsilon"):
-            if hasattr(norm, name):
-                return float(getattr(norm, name))
-        return None
+    _norm_eps = staticmethod(norm_eps)
 
     def _modules_are_fusable(self) -> bool:
         """True when every layer is the plain Ouro block the one-launch glue kernels restate:
@@ -249,6 +260,8 @@ class FlashLoopEngine:
     def _decode_step(self, token_ids: torch.Tensor, position_ids: torch.Tensor) -> torch.Tensor:
         """The device work of one decode step; returns float32 logits [B, vocab]."""
 
+        if self.projection_format is not None:
+            return self._decode_step_microscaled(token_ids, position_ids)
         if self.fuse_decode_ops and token_ids.is_cuda:
             return self._decode_step_fused(token_ids, position_ids)
         return self._decode_step_modules(token_ids, position_ids)
@@ -377,6 +390,52 @@ class FlashLoopEngine:
         for index in range(n_layers):
             cache.layers[index].append_decode_token(keys[index], values[index])
         return self.model.lm_head(hidden[:, -1]).float()  # 200 MB of weights: the library GEMM streams them at 0.88 of peak
+
+    def _decode_step_microscaled(self, token_ids: torch.Tensor, position_ids: torch.Tensor) -> torch.Tensor:
+        """:meth:`_decode_step_fused` with microscaled projections, for any batch: the norms and the gated
+        activation hand their rows on in mxfp8, the readers' float32 output is quantised for ``o_proj``."""
+
+        cache = self.state.cache
+        hidden = self.backbone.embed_tokens(token_ids)
+        batch = int(token_ids.shape[0])
+        cos, sin = self.backbone.rotary_emb(hidden, position_ids)
+        cos, sin = cos.contiguous(), sin.contiguous()
+        n_layers = len(self.layers)
+        keys = [[None] * 4 for _ in range(n_layers)]
+        values = [[None] * 4 for _ in range(n_layers)]
+        sources = [None] * n_layers
+        eps = self._norm_eps
+        first = self.layers[0].input_layernorm
+        for loop in range(4):
+            x = mx_rmsnorm(hidden, first.weight, eps(first))[0]
+            for index, layer in enumerate(self.layers):
+                attention, mlp = layer.self_attn, layer.mlp
+                if loop >= 2 and self._reuse:
+                    v = project_value(attention, x).view(batch, -1, 1, 128)
+                    q, k = None, keys[index][1]
+                else:
+                    q, k, v = step_ops.rope_split(*project_qkv(attention, x), cos, sin,
+                                                  heads=attention._flashloop_qkv_splits[0] // 128)
+                keys[index][loop], values[index][loop] = k, v
+                partial, addend, keep = self._attend(loop, index, q, k, v, float(attention.scaling), sources,
+                                                     lambda t, w=attention._flashloop_mx_output: mx_linear(t, w),
+                                                     batch, convert=False)
+                if keep:
+                    sources[index][0] = partial
+                n2, n3, n4 = layer.input_layernorm_2, layer.post_attention_layernorm, layer.post_attention_layernorm_2
+                x, hidden, _ = mx_rmsnorm(partial, n2.weight, eps(n2), residual=hidden, weight2=n3.weight, eps2=eps(n3),
+                                          addend=addend)
+                m = mx_linear(mx_linear_swiglu(x, mlp._flashloop_mx_gate, mlp._flashloop_mx_up, out_format="mxfp8"),
+                              mlp._flashloop_mx_down)
+                if index < n_layers - 1:
+                    following = self.layers[index + 1].input_layernorm
+                    x, hidden, _ = mx_rmsnorm(m, n4.weight, eps(n4), residual=hidden, weight2=following.weight,
+                                              eps2=eps(following))
+            final = self.backbone.norm  # of this loop: the next one starts from its rows
+            hidden = step_ops.rmsnorm(m, n4.weight, eps(n4), residual=hidden, weight2=final.weight, eps2=eps(final))[1]
+        for index in range(n_layers):
+            cache.layers[index].append_decode_token(keys[index], values[index])
+        return self.model.lm_head(hidden[:, -1]).float()
 
     def _decode_step_modules(self, token_ids: torch.Tensor, position_ids: torch.Tensor) -> torch.Tensor:
         """One decode step through the model's own modules (any Ouro-style block)."""

@@ -3,7 +3,7 @@
 Mirrors flashloop/prefill.py:122-342 (``_execute_prefill_loop``, ``dense_prefill_loop``,
 ``sparse_prefill_loop``, ``PrefillReceipt``): a late loop sends only its retained rows
 through Q/K/V, the output projection and the MLP, while every retained query still attends the
-full causal composite K/V.  The GEMMs and SDPA are library calls; the row movement (gather of
+full causal composite K/V.  The GEMMs (unless the weights are microscaled) and SDPA are library calls; the row movement (gather of
 retained rows, scatter of their results) goes through ``compaction.gather_rows`` /
 ``scatter_rows`` instead of ``index_select`` / ``index_copy_``.
 
@@ -20,8 +20,10 @@ import torch
 from torch import nn
 from torch.nn import functional as F
 
+from . import step_ops
 from .compaction import RetainedTokens, gather_rows, scatter_rows
-from .weights import fused_mlp, project_qkv
+from .mx import mx_rmsnorm
+from .weights import fused_mlp, project_output, project_qkv
 
 
 @dataclass(frozen=True)
@@ -76,7 +78,28 @@ def _identity(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def norm_eps(norm: nn.Module) -> float | None:
+    for name in ("eps", "variance_epsilon"):
+        if hasattr(norm, name):
+            return float(getattr(norm, name))
+    return None
+
+
+def _input_norm(layer: nn.Module, hidden: torch.Tensor):
+    """The rows that Q/K/V project: in mxfp8 where the weights are microscaled."""
+
+    norm = layer.input_layernorm
+    if getattr(layer.self_attn, "_flashloop_mx_qkv", None) is None:
+        return norm(hidden)
+    return mx_rmsnorm(hidden, norm.weight, norm_eps(norm))[0]
+
+
 def _layer_tail(layer: nn.Module, residual: torch.Tensor, attention_output: torch.Tensor, reduce) -> torch.Tensor:
+    if getattr(layer.mlp, "_flashloop_mx_gate", None) is not None:
+        n2, n3, n4 = layer.input_layernorm_2, layer.post_attention_layernorm, layer.post_attention_layernorm_2
+        rows, hidden, _ = mx_rmsnorm(attention_output, n2.weight, norm_eps(n2), residual=residual, weight2=n3.weight,
+                                     eps2=norm_eps(n3))
+        return step_ops.rmsnorm(fused_mlp(layer.mlp, rows), n4.weight, norm_eps(n4), residual=hidden)
     hidden = residual + layer.input_layernorm_2(attention_output)
     mlp_out = reduce(fused_mlp(layer.mlp, layer.post_attention_layernorm(hidden)))
     return hidden + layer.post_attention_layernorm_2(mlp_out)
@@ -94,7 +117,7 @@ def dense_prefill_loop(layers: Sequence[nn.Module], hidden_states: torch.Tensor,
     for layer in layers:
         attention = layer.self_attn
         head_dim = int(attention.head_dim)
-        q, k, v = project_qkv(attention, layer.input_layernorm(hidden))
+        q, k, v = project_qkv(attention, _input_norm(layer, hidden))
         heads = q.shape[-1] // head_dim
         q, k, v = _heads(q, heads, head_dim), _heads(k, heads, head_dim), _heads(v, heads, head_dim)
         q, k = apply_rope(q, k, cos, sin)
@@ -102,7 +125,7 @@ def dense_prefill_loop(layers: Sequence[nn.Module], hidden_states: torch.Tensor,
         keys.append(k)
         values.append(v)
         out = F.scaled_dot_product_attention(q, k, v, dropout_p=0.0, is_causal=True)
-        out = reduce(attention.o_proj(out.transpose(1, 2).reshape(batch, tokens, -1)))
+        out = reduce(project_output(attention, out.transpose(1, 2).reshape(batch, tokens, -1)))
         hidden = _layer_tail(layer, hidden, out, reduce)
     hidden = final_norm(hidden)
     n = len(layers)
@@ -142,7 +165,7 @@ def sparse_prefill_loop(layers: Sequence[nn.Module], hidden_states: torch.Tensor
     for index, layer in enumerate(layers):
         attention = layer.self_attn
         head_dim = int(attention.head_dim)
-        q, k, v = project_qkv(attention, layer.input_layernorm(active))
+        q, k, v = project_qkv(attention, _input_norm(layer, active))
         heads = q.shape[-1] // head_dim
         q, k, v = _heads(q, heads, head_dim), _heads(k, heads, head_dim), _heads(v, heads, head_dim)
         q, k = apply_rope(q, k, cos, sin)
@@ -158,7 +181,7 @@ def sparse_prefill_loop(layers: Sequence[nn.Module], hidden_states: torch.Tensor
         values.append(full_v)
         updates.append((k, v))
         out = F.scaled_dot_product_attention(q, full_k, full_v, attn_mask=attn_mask, dropout_p=0.0)
-        out = reduce(attention.o_proj(out.transpose(1, 2).reshape(batch, rows, -1)))
+        out = reduce(project_output(attention, out.transpose(1, 2).reshape(batch, rows, -1)))
         active = _layer_tail(layer, active, out, reduce)
     active = final_norm(active)
     scatter_rows(hidden, active.contiguous(), positions, count)

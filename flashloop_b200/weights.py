@@ -1,6 +1,7 @@
 """Fused projection weights (flashloop/weights.py:20-117): Q/K/V and gate/up are stored as one
 buffer each so that a decode step issues one GEMM instead of three / two.  The GEMMs themselves
-are library calls (cuBLAS through ``F.linear``)."""
+are library calls (cuBLAS through ``F.linear``), or the microscaled products of :mod:`.mx` once
+:func:`quantize_projection_weights` has replaced the weights."""
 
 from __future__ import annotations
 
@@ -9,6 +10,8 @@ from collections.abc import Sequence
 import torch
 from torch import nn
 from torch.nn import functional as F
+
+from .mx import MXTensor, mx_linear, mx_linear_swiglu, mx_quantize
 
 
 @torch.no_grad()
@@ -38,18 +41,57 @@ def repack_projection_weights(layers: Sequence[nn.Module]) -> None:
             module.weight = None
 
 
-def project_qkv(attention: nn.Module, values: torch.Tensor):
-    """weights.py:74-88."""
+@torch.no_grad()
+def quantize_projection_weights(layers: Sequence[nn.Module], format: str) -> None:
+    """Replace the repacked projection weights of every layer (Q/K/V, ``o_proj``, gate, up,
+    ``down_proj``) by their microscaled form and release the bfloat16 tensors.  No counterpart in the
+    reference, whose projections stay bfloat16 (flashloop/weights.py:20-117)."""
 
+    for layer in layers:
+        attention, mlp = layer.self_attn, layer.mlp
+        done = getattr(attention, "_flashloop_mx_qkv", None)
+        if done is not None:
+            if done.format != format:
+                raise RuntimeError(f"the projections are already held in {done.format}")
+            continue
+        if not hasattr(attention, "_flashloop_qkv_weight") or not hasattr(mlp, "_flashloop_gate_up_weight"):
+            raise ValueError("microscaled projections need fused projection weights (repack_projection_weights)")
+        for name, module in (("o_proj", attention.o_proj), ("down_proj", mlp.down_proj)):
+            if module.bias is not None:
+                raise ValueError(f"microscaled projections require biasless {name}")
+        qkv = mx_quantize(attention._flashloop_qkv_weight, format)
+        value_row = sum(attention._flashloop_qkv_splits[:2])
+        if value_row % 128:
+            raise ValueError("microscaled projections need heads of 128 channels")
+        gate, up = mlp._flashloop_gate_up_weight.split(mlp._flashloop_gate_up_splits, dim=0)
+        attention._flashloop_mx_qkv = qkv
+        attention._flashloop_mx_value = MXTensor(qkv.codes[value_row:], qkv.scales[value_row // 128:],
+                                                 (attention._flashloop_qkv_splits[2], qkv.cols), format)
+        attention._flashloop_mx_output = mx_quantize(attention.o_proj.weight, format)
+        mlp._flashloop_mx_gate, mlp._flashloop_mx_up = mx_quantize(gate, format), mx_quantize(up, format)
+        mlp._flashloop_mx_down = mx_quantize(mlp.down_proj.weight, format)
+        attention._flashloop_qkv_weight = mlp._flashloop_gate_up_weight = None
+        attention.o_proj.weight = mlp.down_proj.weight = None
+
+
+def project_qkv(attention: nn.Module, values):
+    """weights.py:74-88; ``values`` may be an :class:`MXTensor` where the weights are."""
+
+    weight = getattr(attention, "_flashloop_mx_qkv", None)
+    if weight is not None:
+        return tuple(mx_linear(values, weight).split(attention._flashloop_qkv_splits, dim=-1))
     weight = getattr(attention, "_flashloop_qkv_weight", None)
     if weight is None:
         return attention.q_proj(values), attention.k_proj(values), attention.v_proj(values)
     return tuple(F.linear(values, weight).split(attention._flashloop_qkv_splits, dim=-1))
 
 
-def project_value(attention: nn.Module, values: torch.Tensor) -> torch.Tensor:
+def project_value(attention: nn.Module, values) -> torch.Tensor:
     """weights.py:91-105: only V, from the packed QKV weight without copying it."""
 
+    weight = getattr(attention, "_flashloop_mx_value", None)
+    if weight is not None:
+        return mx_linear(values, weight)
     weight = getattr(attention, "_flashloop_qkv_weight", None)
     if weight is None:
         return attention.v_proj(values)
@@ -57,9 +99,21 @@ def project_value(attention: nn.Module, values: torch.Tensor) -> torch.Tensor:
     return F.linear(values, weight.narrow(0, q_features + k_features, v_features))
 
 
-def fused_mlp(mlp: nn.Module, values: torch.Tensor) -> torch.Tensor:
-    """weights.py:108-117."""
+def project_output(attention: nn.Module, values: torch.Tensor) -> torch.Tensor:
+    """The ``o_proj`` call of flashloop/prefill.py and flashloop/engine.py:531."""
 
+    weight = getattr(attention, "_flashloop_mx_output", None)
+    return attention.o_proj(values) if weight is None else mx_linear(values, weight)
+
+
+def fused_mlp(mlp: nn.Module, values) -> torch.Tensor:
+    """weights.py:108-117; with microscaled weights the gated activation stays in mxfp8 on its way to
+    the down projection."""
+
+    gate = getattr(mlp, "_flashloop_mx_gate", None)
+    if gate is not None:
+        return mx_linear(mx_linear_swiglu(values, gate, mlp._flashloop_mx_up, out_format="mxfp8"),
+                         mlp._flashloop_mx_down)
     weight = getattr(mlp, "_flashloop_gate_up_weight", None)
     if weight is None:
         return mlp(values)

@@ -116,3 +116,12 @@ def test_c_refusals(lib):
     assert lib.fl_mx_linear_swiglu(a, a, 0, a, a, a, None, 1, 4, 64, 64, a, 0, 0, None, None) == -1 and "null" in last()
     assert lib.fl_mx_linear_swiglu(a, a, 0, a, a, a, a, 1, 4, 64, 64, a, 0, 4, a, None) == -1 and "output" in last()
     assert lib.fl_mx_status(None, 0, None) == -1
+
+
+def test_engine_refusals_on_the_host():
+    from tests.helpers import tiny_ouro_model
+
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        fl.FlashLoopEngine(tiny_ouro_model(), validate_model=False, projection_format="mxfp4")
+    with pytest.raises(ValueError, match="tensor parallelism"):
+        fl.FlashLoopEngine(tiny_ouro_model(), validate_model=False, projection_format="mxfp4", tp_group=object())
