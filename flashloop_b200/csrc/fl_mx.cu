@@ -19,6 +19,8 @@ quantize_kernel(const T* __restrict__ x, uint32_t rows, int cols, int64_t row_st
   const uint32_t first = blockIdx.x * (UNROLL * kMxThreads / 8) + threadIdx.x / 8;
   const int lane = threadIdx.x & 7;
   __shared__ __align__(16) WarpStage<T, VEC, kMxThreads> stage;
+  wait_for_inputs();
+  may_start_next();
   Raw16<T> raw[UNROLL];
   uint32_t row[UNROLL];
   int e[UNROLL];
@@ -55,6 +57,8 @@ dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
   const uint32_t first = blockIdx.x * (UNROLL * kMxThreads / 8) + threadIdx.x / 8;
   const int lane = threadIdx.x & 7;
   __shared__ __align__(16) WarpStage<T, VEC, kMxThreads> stage;
+  wait_for_inputs();
+  may_start_next();
   uint4 word[UNROLL] = {};
   uint32_t byte[UNROLL] = {};
   uint32_t row[UNROLL];
@@ -185,6 +189,8 @@ __global__ void __launch_bounds__(kNormThreads<WARPS>) norm_mx_kernel(const MxNo
   const int64_t stride = int64_t(gridDim.x) * kRows;
   const bool one_group = p.rows <= 32;  // a row's word is then the only one of its sixteen bytes
   int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / kRowThreads;
+  wait_for_inputs();
+  may_start_next();
   NormRow<T, CHUNKS, SECOND> next;
   next.template load<VEC, kRowThreads>(p, row, thread, stage.mine());
   float w[CHUNKS][16], w2[SECOND ? CHUNKS : 1][16];
@@ -280,22 +286,14 @@ __global__ void __launch_bounds__(kNormThreads<WARPS>) norm_mx_kernel(const MxNo
   }
 }
 
-// Rounds per thread: four where that still leaves several CTAs to an SM, one below.
+// Rounds per thread: several where that still leaves several CTAs to an SM, one below.
 constexpr int64_t kUnrollUnits = 148 * 8 * 64;
 
-template <typename T, int FORMAT, bool VEC>
-void launch_quantize(const T* x, int64_t rows, int32_t cols, int64_t stride, uint32_t steps, uint32_t units, void* codes,
-                     void* scales, cudaStream_t stream) {
-  uint8_t* c = static_cast<uint8_t*>(codes);
-  uint8_t* s = static_cast<uint8_t*>(scales);
-  constexpr int kUnits = kMxThreads / 8;
-  if (units >= kUnrollUnits) {
-    quantize_kernel<T, FORMAT, VEC, 2><<<(units + 2 * kUnits - 1) / (2 * kUnits), kMxThreads, 0, stream>>>(
-        x, uint32_t(rows), cols, stride, steps, units, c, s);
-  } else {
-    quantize_kernel<T, FORMAT, VEC, 1><<<(units + kUnits - 1) / kUnits, kMxThreads, 0, stream>>>(
-        x, uint32_t(rows), cols, stride, steps, units, c, s);
-  }
+int launched(cudaError_t err, const char* who) {
+  if (err == cudaSuccess) return FL_OK;
+  cudaGetLastError();
+  set_error("%s: %s", who, cudaGetErrorString(err));
+  return FL_ERR_CUDA;
 }
 
 template <typename T, int FORMAT>
@@ -304,14 +302,14 @@ int launch_quantize(const void* x, int64_t rows, int32_t cols, int64_t stride, v
   const int64_t steps = mx_steps(cols);
   const int64_t units = (rows + kMxTileRows - 1) / kMxTileRows * kMxTileRows * steps;
   FL_REQUIRE(units < (int64_t(1) << 31), "fl_mx_quantize: too many elements");
-  const T* src = static_cast<const T*>(x);
-  if (aligned16(x) && (stride * sizeof(T) % 16 == 0 || rows == 1)) {
-    launch_quantize<T, FORMAT, true>(src, rows, cols, stride, uint32_t(steps), uint32_t(units), codes, scales, stream);
-  } else {
-    launch_quantize<T, FORMAT, false>(src, rows, cols, stride, uint32_t(steps), uint32_t(units), codes, scales, stream);
-  }
-  FL_CHECK_LAUNCH("fl_mx_quantize");
-  return FL_OK;
+  const bool vec = aligned16(x) && (stride * sizeof(T) % 16 == 0 || rows == 1), many = units >= kUnrollUnits;
+  auto kernel = many ? (vec ? quantize_kernel<T, FORMAT, true, 2> : quantize_kernel<T, FORMAT, false, 2>)
+                     : (vec ? quantize_kernel<T, FORMAT, true, 1> : quantize_kernel<T, FORMAT, false, 1>);
+  const int64_t each = (many ? 2 : 1) * (kMxThreads / 8);
+  return launched(launch_overlapped(kernel, unsigned((units + each - 1) / each), kMxThreads, 0, 1, stream,
+                                    static_cast<const T*>(x), uint32_t(rows), cols, stride, uint32_t(steps), uint32_t(units),
+                                    static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales)),
+                  "fl_mx_quantize");
 }
 
 template <typename T, int FORMAT>
@@ -326,10 +324,9 @@ int launch_dequantize(const void* codes, const void* scales, int64_t rows, int32
   auto kernel = many ? (vec ? dequantize_kernel<T, FORMAT, true, 4> : dequantize_kernel<T, FORMAT, false, 4>)
                      : (vec ? dequantize_kernel<T, FORMAT, true, 1> : dequantize_kernel<T, FORMAT, false, 1>);
   const int64_t each = many ? 4 * kUnits : kUnits;
-  kernel<<<unsigned((units + each - 1) / each), kMxThreads, 0, stream>>>(c, s, cols, uint32_t(steps), uint32_t(units),
-                                                                        static_cast<T*>(out));
-  FL_CHECK_LAUNCH("fl_mx_dequantize");
-  return FL_OK;
+  return launched(launch_overlapped(kernel, unsigned((units + each - 1) / each), kMxThreads, 0, 1, stream, c, s, cols,
+                                    uint32_t(steps), uint32_t(units), static_cast<T*>(out)),
+                  "fl_mx_dequantize");
 }
 
 struct NormArgs {
@@ -341,15 +338,15 @@ struct NormArgs {
 };
 
 template <typename T, int FORMAT, bool VEC, bool SECOND, int WARPS, int CHUNKS>
-void launch_norm_shape(const MxNormParams<T>& p, cudaStream_t stream) {
+cudaError_t launch_norm_shape(const MxNormParams<T>& p, cudaStream_t stream) {
   constexpr int kThreads = kNormThreads<WARPS>, kRows = kThreads / 32 / WARPS;
   const int64_t ctas = std::min<int64_t>((p.rows + kRows - 1) / kRows, 148 * ((SECOND ? kNormSmThreads2 : kNormSmThreads) / kThreads));
-  norm_mx_kernel<T, FORMAT, VEC, SECOND, WARPS, CHUNKS><<<unsigned(ctas), kThreads, 0, stream>>>(p);
+  return launch_overlapped(norm_mx_kernel<T, FORMAT, VEC, SECOND, WARPS, CHUNKS>, unsigned(ctas), kThreads, 0, 1, stream, p);
 }
 
 // Warps to a row: as few as hold it once there are rows enough to fill the SMs, otherwise eight.
 template <typename T, int FORMAT, bool VEC, bool SECOND>
-void launch_norm_rows(const MxNormParams<T>& p, cudaStream_t stream) {
+cudaError_t launch_norm_rows(const MxNormParams<T>& p, cudaStream_t stream) {
   const bool many = p.rows >= kManyRows;
   if (many && p.width <= 512) return launch_norm_shape<T, FORMAT, VEC, SECOND, 1, 1>(p, stream);
   if (many && p.width <= 1024) return launch_norm_shape<T, FORMAT, VEC, SECOND, 2, 1>(p, stream);
@@ -378,13 +375,13 @@ int launch_norm(const NormArgs& a, cudaStream_t stream) {
   const bool vec = aligned16(a.x) && aligned16(a.addend) && aligned16(a.residual) && aligned16(a.weight) &&
                    aligned16(a.weight2) && aligned16(a.sum_out) && aligned16(a.hidden) &&
                    a.width * sizeof(T) % 16 == 0;
+  cudaError_t err;
   if (vec) {
-    a.weight2 ? launch_norm_rows<T, FORMAT, true, true>(p, stream) : launch_norm_rows<T, FORMAT, true, false>(p, stream);
+    err = a.weight2 ? launch_norm_rows<T, FORMAT, true, true>(p, stream) : launch_norm_rows<T, FORMAT, true, false>(p, stream);
   } else {
-    a.weight2 ? launch_norm_rows<T, FORMAT, false, true>(p, stream) : launch_norm_rows<T, FORMAT, false, false>(p, stream);
+    err = a.weight2 ? launch_norm_rows<T, FORMAT, false, true>(p, stream) : launch_norm_rows<T, FORMAT, false, false>(p, stream);
   }
-  FL_CHECK_LAUNCH("fl_rmsnorm_mx");
-  return FL_OK;
+  return launched(err, "fl_rmsnorm_mx");
 }
 
 // Calls f.template run<T, FORMAT>() for the type and format codes (validated by the caller).

@@ -12,6 +12,7 @@
 
 #include <cstring>
 #include <type_traits>
+#include <utility>
 
 #include "fl_common.cuh"
 
@@ -30,6 +31,33 @@ constexpr int64_t mx_row_bytes(int64_t cols, int format) {
 inline bool mx_format_ok(int format) { return format == FL_MX_FP8 || format == FL_MX_FP4; }
 
 #ifdef __CUDACC__
+
+// The kernels on microscaled tensors are launched so that they may start while the kernel before them
+// in the stream is ending (programmatic dependent launch).  They read and write nothing of the caller's
+// before wait_for_inputs(), which every thread passes and which returns when all earlier work of the stream is
+// done and visible; what comes before it is their own set-up.  may_start_next() lets the next such
+// kernel set up once all CTAs of this one run.
+__device__ __forceinline__ void wait_for_inputs() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void may_start_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+cudaError_t launch_overlapped(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem, unsigned cluster,
+                              cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(block);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = cluster;
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+  config.attrs = attributes;
+  config.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...);
+}
 
 // Byte offset of the scale of (row, step, block 0 of the step).
 __device__ __forceinline__ int64_t mx_scale_offset(int64_t row, int64_t step, int64_t steps) {

@@ -148,6 +148,9 @@ __device__ __forceinline__ void send16(uint32_t cluster_addr, const uint32_t* v,
   asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
                ::"r"(cluster_addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(cluster_bar) : "memory");
 }
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p) : "memory");
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
@@ -225,7 +228,8 @@ __device__ __forceinline__ void zero_scales(const Output& o, int64_t rows, int n
 }
 
 struct LinearParams {
-  const uint8_t *x_scales, *w_scales[2];
+  const uint8_t *x_scales, *w_scales[2], *w_codes[2];
+  int w_row_step;  // bytes of a row of the weight's codes per step
   Output out;
   int64_t rows;
   int steps;   // of K
@@ -297,8 +301,27 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       prefetch_map(&map_x);
       if (DUAL) prefetch_map(&map_w1);
     }
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                 "r"(p.tmem_cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  // The weight on its way into the L2 cache, which is harmless whoever still writes it.
+  {
+    const int row_lines = ((last - first) * p.w_row_step + 127) / 128;
+    for (int i = threadIdx.x; i < 128 * row_lines; i += kLinThreads) {
+      const int row = w_tile * 128 + i / row_lines;
+      const int64_t at = (int64_t(row) * p.steps + first) * p.w_row_step + i % row_lines * 128;
+      if (row < p.out.features) {
+        prefetch_l2(p.w_codes[0] + at);
+        if (DUAL) prefetch_l2(p.w_codes[1] + at);
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  wait_for_inputs();
+  may_start_next();
   if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA runs
 
   if (warp == 0 || (warp >= 2 && warp <= 4)) {
@@ -331,12 +354,7 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       __syncwarp();
     }
   } else if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
-                 "r"(p.tmem_cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    __syncwarp();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    asm volatile("bar.arrive 1, 160;" ::: "memory");  // the epilogue may read the slot
     const uint32_t tmem_scales = tmem + NT * kWeights;
     // scales of x: NT rows of a 128-row tile start at its column (row0 % 128) / 32, an even one
     const uint32_t x_col = 4 * kWeights + uint32_t(row0 % kMxTileRows) / 32;
@@ -375,7 +393,6 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   const int n = w_tile * 128 + (warp & 3) * 32 + lane;
   const bool features_whole = w_tile * 128 + 128 <= p.out.features;
   if (warp >= 2) {
-    asm volatile("bar.sync 1, 160;" ::: "memory");
     const uint32_t acc = __shfl_sync(0xffffffffu, *tmem_slot, 0) + (uint32_t(warp & 3) * 32 << 16);
     mbar_wait(done, 0);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -550,6 +567,8 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   cluster_sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  wait_for_inputs();
+  may_start_next();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const uint32_t tmem_scales = tmem + 2 * kPairRows;
 
@@ -768,6 +787,9 @@ int launch_linear(const LinearCall& call, int splits, int most_stages) {
   p.x_scales = static_cast<const uint8_t*>(call.x.scales);
   p.w_scales[0] = static_cast<const uint8_t*>(call.w[0].scales);
   p.w_scales[1] = static_cast<const uint8_t*>(call.w[1].scales);
+  p.w_codes[0] = static_cast<const uint8_t*>(call.w[0].codes);
+  p.w_codes[1] = static_cast<const uint8_t*>(call.w[1].codes);
+  p.w_row_step = call.w[0].format == FL_MX_FP8 ? kMxStep : kMxStep / 2;
   p.out = Output{call.out, static_cast<uint8_t*>(call.out_scales), call.features, (call.features + 127) / 128};
   p.rows = call.rows;
   p.steps = steps;
@@ -799,18 +821,8 @@ int launch_linear(const LinearCall& call, int splits, int most_stages) {
   auto kernel = mx_linear_kernel<KIND, NT, DUAL>;
   static std::atomic<bool> allowed[kMaxDevices];
   cudaError_t err = allow_shared_memory(kernel, allowed, call.device);
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(unsigned(tiles * splits));
-  config.blockDim = dim3(kLinThreads);
-  config.dynamicSmemBytes = smem;
-  config.stream = call.stream;
-  cudaLaunchAttribute attribute;
-  attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = splits;
-  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
-  if (err == cudaSuccess) err = cudaLaunchKernelEx(&config, kernel, map_x, map_w0, map_w1, p);
+  if (err == cudaSuccess)
+    err = launch_overlapped(kernel, unsigned(tiles * splits), kLinThreads, smem, splits, call.stream, map_x, map_w0, map_w1, p);
   if (err != cudaSuccess) {
     cudaGetLastError();
     set_error("%s: %s", call.who, cudaGetErrorString(err));
@@ -865,18 +877,10 @@ int launch_pairs(const LinearCall& call, int sms) {
   auto kernel = mx_linear_pair_kernel<KIND, DUAL>;
   static std::atomic<bool> allowed[kMaxDevices];
   cudaError_t err = allow_shared_memory(kernel, allowed, call.device);
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(unsigned(2 * std::min<int64_t>(tiles, sms / 2)));
-  config.blockDim = dim3(kPairThreads);
-  config.dynamicSmemBytes = kSmemLimit;  // all of an SM's, as it takes all of its tensor memory (see above)
-  config.stream = call.stream;
-  cudaLaunchAttribute attribute;
-  attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = 2;
-  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
-  if (err == cudaSuccess) err = cudaLaunchKernelEx(&config, kernel, maps, p);
+  // all of an SM's shared memory, as it takes all of its tensor memory (see above)
+  if (err == cudaSuccess)
+    err = launch_overlapped(kernel, unsigned(2 * std::min<int64_t>(tiles, sms / 2)), kPairThreads, kSmemLimit, 2, call.stream,
+                            maps, p);
   if (err != cudaSuccess) {
     cudaGetLastError();
     set_error("%s: %s", call.who, cudaGetErrorString(err));
