@@ -32,6 +32,7 @@ constexpr int kMaxStages = 12;
 constexpr int kMaxSplits = 8;
 constexpr int kSmemLimit = 232448;
 constexpr int kSmemPerSm = 233472;
+constexpr int kSmemHalf = kSmemPerSm / 2 - 1024;
 constexpr int kTailBytes = 512;  // barriers and the tensor memory base
 
 __device__ int g_mx_status;
@@ -780,7 +781,7 @@ struct LinearCall {
 };
 
 template <int KIND, int NT, bool DUAL>
-int launch_linear(const LinearCall& call, int splits, int most_stages) {
+int launch_linear(const LinearCall& call, int splits, int smem_limit) {
   using Shape = FewRows<NT, DUAL>;
   const int steps = int(mx_steps(call.cols));
   LinearParams p;
@@ -796,8 +797,8 @@ int launch_linear(const LinearCall& call, int splits, int most_stages) {
   p.w_bytes = uint32_t(kTileW >> (call.w[0].format == FL_MX_FP8 ? 0 : 1));
   p.x_bytes = uint32_t(Shape::kXBytes >> (call.x.format == FL_MX_FP8 ? 0 : 1));
   const int exchange = Shape::exchange_bytes(splits, int(std::min<int64_t>(NT, call.rows)));
-  const int room = (kSmemLimit - 1024 - kTailBytes - exchange) / Shape::kStageBytes;
-  p.stages = std::min({kMaxStages, room, most_stages, (steps + splits - 1) / splits});
+  const int room = (smem_limit - 1024 - kTailBytes - exchange) / Shape::kStageBytes;
+  p.stages = std::min({kMaxStages, room, (steps + splits - 1) / splits});
   const int need = NT * Shape::kWeights + p.stages * int(Shape::kScaleCols);
   p.tmem_cols = need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
   // Shared memory in proportion to the columns: CTAs of these kernels that fit an SM together
@@ -889,11 +890,11 @@ int launch_pairs(const LinearCall& call, int sms) {
   return FL_OK;
 }
 
-// Multiprocessors of a device and, for every cluster size, how many clusters of CTAs that fill an SM each run
-// at once (the GPU's processor groups do not divide evenly).
+// Multiprocessors of a device and, for every cluster size, how many clusters run at once of CTAs that take
+// all of an SM's shared memory and of CTAs that take half (the GPU's processor groups do not divide evenly).
 struct Device {
   int sms;
-  int clusters[kMaxSplits + 1];
+  int clusters[2][kMaxSplits + 1];
 };
 const Device& device_limits(int device) {
   static Device limits[kMaxDevices];
@@ -904,46 +905,57 @@ const Device& device_limits(int device) {
     if (cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || d.sms <= 0) d.sms = 148;
     auto kernel = mx_linear_kernel<kOutBf16, 16, false>;
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
-    for (int size = 1; size <= kMaxSplits; ++size) {
-      cudaLaunchConfig_t config{};
-      config.gridDim = dim3(unsigned(size));
-      config.blockDim = dim3(kLinThreads);
-      config.dynamicSmemBytes = kSmemLimit;
-      cudaLaunchAttribute attribute;
-      attribute.id = cudaLaunchAttributeClusterDimension;
-      attribute.val.clusterDim.x = size;
-      attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-      config.attrs = &attribute;
-      config.numAttrs = 1;
-      if (cudaOccupancyMaxActiveClusters(&d.clusters[size], kernel, &config) != cudaSuccess) d.clusters[size] = 0;
+    for (int half = 0; half < 2; ++half) {
+      for (int size = 1; size <= kMaxSplits; ++size) {
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(unsigned(size));
+        config.blockDim = dim3(kLinThreads);
+        config.dynamicSmemBytes = half ? kSmemHalf : kSmemLimit;
+        cudaLaunchAttribute attribute;
+        attribute.id = cudaLaunchAttributeClusterDimension;
+        attribute.val.clusterDim.x = size;
+        attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+        config.attrs = &attribute;
+        config.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&d.clusters[half][size], kernel, &config) != cudaSuccess)
+          d.clusters[half][size] = 0;
+      }
     }
     cudaGetLastError();
   });
   return limits[device];
 }
 
+// How a call is cut, by its tiles of 128 features by NT rows and its steps of K:
+// - up to 32 rows, CTAs take half of an SM's shared memory, so that two fit an SM and the next kernel's can set up beside
+//   the last ones of this; K is split while that gives at most three CTAs to two SMs and three steps to a CTA
+//   (16 rows, mxfp4, weights not in L2; 2048 -> 6144: split two ways with all of the shared memory 4.7 us, two ways
+//   with half 4.8, three 4.4, four 4.1, five 4.5; 2048 -> 2048: four 3.4, six 3.3, eight 3.4; 5632 -> 2048: four
+//   5.2, six 4.5, eight 4.3; gated 2048 -> 5632: two with all 7.0, three with all 6.7, five with half 6.5);
+// - with more rows the exchange of the sums weighs more: two CTAs to three SMs, each taking all of its shared memory
+//   (64 rows, 2048 -> 6144: two ways 6.5 us, three 7.9);
+// - never more than run at once: a cluster that waits for another to end doubles the call (2048 -> 6144
+//   split three ways with all of the shared memory: 7.8 us).
 template <int KIND, bool DUAL>
 int choose_linear(const LinearCall& call) {
   const Device& device = device_limits(call.device);
   const int sms = device.sms;
   const int steps = int(mx_steps(call.cols));
   const int64_t w_tiles = (call.features + 127) / 128;
-  // The widest split whose clusters all run at once: more CTAs read the weight, until a cluster has to wait
-  // for another to end (16 rows, mxfp4; 2048 -> 6144: one CTA a tile 6.6 us, two 5.4, three, of which
-  // not all fit, 8.3; 2048 -> 2048: one 6.5, four 4.4, six 4.2, eight, of which not all fit, 5.3).
   auto splits_for = [&](int nt) {
+    const bool half = nt <= 32;
     const int64_t tiles = (call.rows + nt - 1) / nt * w_tiles;
-    int splits = std::min(kMaxSplits, steps);
-    while (splits > 1 && tiles > device.clusters[splits]) --splits;
+    int splits = std::max(1, std::min(kMaxSplits, (steps + 2) / 3));
+    while (splits > 1 && (tiles * splits > (half ? sms * 3 / 2 : sms * 2 / 3) || tiles > device.clusters[half][splits])) --splits;
     return splits;
   };
-  if (call.rows <= 16) return launch_linear<KIND, 16, DUAL>(call, splits_for(16), kMaxStages);
-  if (call.rows <= 32) return launch_linear<KIND, 32, DUAL>(call, splits_for(32), kMaxStages);
-  if (call.rows <= 64) return launch_linear<KIND, 64, DUAL>(call, splits_for(64), kMaxStages);
+  if (call.rows <= 16) return launch_linear<KIND, 16, DUAL>(call, splits_for(16), kSmemHalf);
+  if (call.rows <= 32) return launch_linear<KIND, 32, DUAL>(call, splits_for(32), kSmemHalf);
+  if (call.rows <= 64) return launch_linear<KIND, 64, DUAL>(call, splits_for(64), kSmemLimit);
   if ((call.rows + kPairRows - 1) / kPairRows * ((call.features + 255) / 256) >= sms / 2)
     return launch_pairs<KIND, DUAL>(call, sms);
   constexpr int kTile = DUAL ? 64 : 128;
-  return launch_linear<KIND, kTile, DUAL>(call, splits_for(kTile), kMaxStages);
+  return launch_linear<KIND, kTile, DUAL>(call, splits_for(kTile), kSmemLimit);
 }
 
 template <bool DUAL>
