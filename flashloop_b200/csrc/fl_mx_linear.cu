@@ -935,7 +935,10 @@ const Device& device_limits(int device) {
 // - with more rows the exchange of the sums weighs more: two CTAs to three SMs, each taking all of its shared memory
 //   (64 rows, 2048 -> 6144: two ways 6.5 us, three 7.9);
 // - never more than run at once: a cluster that waits for another to end doubles the call (2048 -> 6144
-//   split three ways with all of the shared memory: 7.8 us).
+//   split three ways with all of the shared memory: 7.8 us);
+// - pairs of CTAs once tiles of 128 rows (64 of a gated product) no longer run at once (2048 -> 6144: 384 rows 8.5 us
+//   either way, 512 rows 15.0 in tiles and 9.0 in pairs, 256 rows 7.8 and 8.8; gated 2048 -> 5632: 192 rows 13.0
+//   and 18.3, 256 rows 24.2 and 18.2).
 template <int KIND, bool DUAL>
 int choose_linear(const LinearCall& call) {
   const Device& device = device_limits(call.device);
@@ -952,9 +955,8 @@ int choose_linear(const LinearCall& call) {
   if (call.rows <= 16) return launch_linear<KIND, 16, DUAL>(call, splits_for(16), kSmemHalf);
   if (call.rows <= 32) return launch_linear<KIND, 32, DUAL>(call, splits_for(32), kSmemHalf);
   if (call.rows <= 64) return launch_linear<KIND, 64, DUAL>(call, splits_for(64), kSmemLimit);
-  if ((call.rows + kPairRows - 1) / kPairRows * ((call.features + 255) / 256) >= sms / 2)
-    return launch_pairs<KIND, DUAL>(call, sms);
   constexpr int kTile = DUAL ? 64 : 128;
+  if ((call.rows + kTile - 1) / kTile * w_tiles > sms) return launch_pairs<KIND, DUAL>(call, sms);
   return launch_linear<KIND, kTile, DUAL>(call, splits_for(kTile), kSmemLimit);
 }
 

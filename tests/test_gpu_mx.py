@@ -193,7 +193,7 @@ def _accumulation(cols):
 
 SIZES = [(1, 1, 1), (1, 32, 128), (2, 128, 130), (16, 2048, 2048), (15, 1000, 1337), (17, 129, 64), (33, 300, 257),
          (64, 512, 384), (65, 4096, 256), (128, 128, 127), (129, 640, 513), (300, 2048, 640), (1000, 160, 4999),
-         (2500, 264, 3000)]
+         (2500, 264, 3000), (3, 20000, 200), (19500, 96, 100), (9800, 300, 200)]
 
 
 @pytest.mark.parametrize("rows,cols,features", SIZES)
@@ -340,6 +340,42 @@ def test_two_streams_and_repeats_agree():
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in got)
     assert mx_status() == 0
+
+
+def test_chains_without_waiting():
+    """The kernels of a chain overlap and its buffers are reused at once: the results are those of the same
+    calls made one by one, for few rows and for many, and with other kernels in between."""
+
+    for rows, width in ((16, 1024), (3, 640), (2000, 512)):
+        g = _gen("chain", rows)
+        inputs = [torch.randn(rows, width, generator=g, device="cuda").to(torch.bfloat16) for _ in range(6)]
+        weight = torch.ones(width, device="cuda", dtype=torch.bfloat16)
+        w = [torch.randn(width, width, generator=g, device="cuda") * width ** -0.5 for _ in range(3)]
+        x = torch.empty_like(inputs[0])
+
+        def chain(values, wait):
+            x.copy_(values)
+            done = lambda t: torch.cuda.synchronize() if wait else None
+            gate, up, down = (fl.mx_quantize(t, "mxfp4") for t in w)  # used by the very next kernels
+            done(gate)
+            out = x
+            for _ in range(4):
+                q, hidden, _ = fl.mx_rmsnorm(out, weight, 1e-6, residual=x, weight2=weight, eps2=1e-6)
+                done(q)
+                inner = fl.mx_linear_swiglu(q, gate, up, out_format="mxfp8")
+                done(inner)
+                out = fl.mx_linear(inner, down)
+                done(out)
+                out = out + hidden  # a kernel of another kind
+                done(out)
+            x.zero_()  # written while the chain may still run, were it not in order
+            return out
+
+        want = [chain(v, True) for v in inputs]
+        torch.cuda.synchronize()
+        for _ in range(5):
+            got = [chain(v, False) for v in inputs]
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_gradients_are_refused():
