@@ -141,6 +141,14 @@ __device__ __forceinline__ float row_sum(float v, float* part) {
   return total;
 }
 
+// In four chains: shorter, and each rounds to less.
+__device__ __forceinline__ float sum_of_squares(const float (&v)[16]) {
+  float s[4] = {};
+#pragma unroll
+  for (int k = 0; k < 16; ++k) s[k & 3] = fmaf(v[k], v[k], s[k & 3]);
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
 // 1 / sqrt(mean + eps): the hardware's root and one Newton step, so that the float32 result carries the rounding
 // of its products only.
 __device__ __forceinline__ float inverse_root(float sum, int width, float eps) {
@@ -219,8 +227,7 @@ __global__ void __launch_bounds__(kNormThreads<WARPS>) norm_mx_kernel(const MxNo
         for (int k = 0; k < 16; ++k) v[c][k] += a[k];
         store16<T, VEC>(p.sum_out + base + e, p.sum_out ? n : 0, v[c], stage.mine());
       }
-#pragma unroll
-      for (int k = 0; k < 16; ++k) sq = fmaf(v[c][k], v[c][k], sq);
+      sq += sum_of_squares(v[c]);
     }
     float inv = inverse_root(row_sum<WARPS>(sq, s_part[0]), p.width, p.eps);
     sq = 0.f;
@@ -235,8 +242,7 @@ __global__ void __launch_bounds__(kNormThreads<WARPS>) norm_mx_kernel(const MxNo
       if constexpr (SECOND) {
         const int e = (c * kRowThreads + thread) * 16, n = live ? p.width - e : 0;
         store16<T, VEC>(p.hidden + base + e, n, v[c], stage.mine());
-#pragma unroll
-        for (int k = 0; k < 16; ++k) sq = fmaf(v[c][k], v[c][k], sq);
+        sq += sum_of_squares(v[c]);
       }
     }
     // one barrier per round orders the reads of s_part[0] before its next writes, and the second sum's does s_part[1]

@@ -189,17 +189,24 @@ __device__ __forceinline__ void emit_rows(const Output& o, int64_t m, int n, con
     const int lane = threadIdx.x & 31;
     const int64_t row_bytes = int64_t(o.w_tiles) * (KIND == kOutFp8 ? kMxStep : kMxStep / 2);
     float q[N];
-    uint32_t mine = 0;  // the scale of row `lane`
+    uint32_t mine = 0;  // the largest magnitude of row `lane`, which works out its scale for all
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       q[j] = live && (WHOLE || j < count) ? v[j] : 0.f;
       const uint32_t amax = __reduce_max_sync(0xffffffffu, __float_as_uint(q[j]) & 0x7fffffffu);
-      const uint32_t byte = mx_scale_byte<kFormat>(amax);
-      q[j] = byte == 255u ? 0.f : q[j] * mx_inverse(byte);
-      mine = lane == j ? byte : mine;
+      mine = lane == j ? amax : mine;
+    }
+    const uint32_t byte = mx_scale_byte<kFormat>(mine);
+    const float inv = mx_inverse(byte);
+    const uint32_t bad = __ballot_sync(0xffffffffu, byte == 255u);
+#pragma unroll
+    for (int j = 0; j < N; ++j) q[j] *= __shfl_sync(0xffffffffu, inv, j);
+    if (bad != 0) {  // a block that is not finite has codes 0
+#pragma unroll
+      for (int j = 0; j < N; ++j) q[j] = bad >> j & 1 ? 0.f : q[j];
     }
     if (lane < (WHOLE ? N : min(N, count)))
-      o.scales[mx_scale_offset(m, n / kMxStep, o.w_tiles) + lane * 16 + n / kMxBlock % 4] = uint8_t(mine);
+      o.scales[mx_scale_offset(m, n / kMxStep, o.w_tiles) + lane * 16 + n / kMxBlock % 4] = uint8_t(byte);
     if constexpr (KIND == kOutFp8) {
       // The codes of four rows in a word, then a 4 x 4 transposition of bytes within each four lanes: a lane
       // has four features of row (lane % 4) and stores them at once.

@@ -157,14 +157,22 @@ def _values(x: torch.Tensor, *others: torch.Tensor | None) -> None:
 
     if x.dtype not in _native.DTYPE_CODES:
         raise TypeError("microscaled operators take bfloat16, float16 or float32")
-    device = x.device
-    _require_cuda(device)
+    if not x.is_cuda:
+        _require_cuda(x.device)
+    index = x.get_device()
+    grad = torch.is_grad_enabled()
     for t in others:
-        if t is not None and t.device != device:
-            _require_cuda(t.device)
-            raise ValueError("all operands must be on one device")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, *others)):
-        raise RuntimeError("microscaled operators record no gradient: call them under torch.no_grad()")
+        if t is not None:
+            if t.get_device() != index:
+                _require_cuda(t.device)
+                raise ValueError("all operands must be on one device")
+            if grad and t.requires_grad:
+                raise RuntimeError(_NO_GRADIENT)
+    if grad and x.requires_grad:
+        raise RuntimeError(_NO_GRADIENT)
+
+
+_NO_GRADIENT = "microscaled operators record no gradient: call them under torch.no_grad()"
 
 
 def mx_quantize(x: torch.Tensor, format: str = "mxfp8") -> MXTensor:
@@ -213,8 +221,10 @@ def mx_rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: t
     if want_sum and addend is None:
         raise ValueError("want_sum needs an addend")
     x = x.contiguous()
-    residual = None if residual is None else residual.contiguous()
-    addend = None if addend is None else addend.contiguous()
+    if residual is not None:
+        residual = residual.contiguous()
+    if addend is not None:
+        addend = addend.contiguous()
     rows = x.numel() // width
     q = MXTensor._empty(shape, rows, format, x)
     hidden = None if weight2 is None else torch.empty_like(x)
