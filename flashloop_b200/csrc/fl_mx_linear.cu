@@ -32,7 +32,7 @@ constexpr int kMaxStages = 12;
 constexpr int kMaxSplits = 8;
 constexpr int kSmemLimit = 232448;
 constexpr int kSmemPerSm = 233472;
-constexpr int kSmemHalf = kSmemPerSm / 2 - 1024;
+constexpr int kSmemHalf = 112 * 1024;  // with the 1 KB that the system takes of each CTA, two fit an SM
 constexpr int kTailBytes = 512;  // barriers and the tensor memory base
 
 __device__ int g_mx_status;
@@ -897,6 +897,10 @@ int launch_pairs(const LinearCall& call, int sms) {
   return FL_OK;
 }
 
+// Never launched: asked about for the kernels below, for which the driver counts one CTA to an SM
+// whatever their shared memory, although two run there (as seen from %smid and %globaltimer).
+__global__ void __launch_bounds__(kLinThreads) cluster_probe_kernel() {}
+
 // Multiprocessors of a device and, for every cluster size, how many clusters run at once of CTAs that take
 // all of an SM's shared memory and of CTAs that take half (the GPU's processor groups do not divide evenly).
 struct Device {
@@ -910,7 +914,7 @@ const Device& device_limits(int device) {
     Device& d = limits[device];
     d.sms = 0;
     if (cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || d.sms <= 0) d.sms = 148;
-    auto kernel = mx_linear_kernel<kOutBf16, 16, false>;
+    auto kernel = cluster_probe_kernel;
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
     for (int half = 0; half < 2; ++half) {
       for (int size = 1; size <= kMaxSplits; ++size) {
