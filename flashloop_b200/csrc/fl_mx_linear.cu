@@ -26,7 +26,8 @@ namespace fl {
 namespace {
 
 constexpr int kLinThreads = 192;
-constexpr int kWaitTries = 1 << 15;
+constexpr int kWaitTries = 1 << 15;  // of one wait, and for every step of K that it may have to sit through:
+constexpr int kWaitTriesPerStep = 256;
 constexpr int kTileW = 128 * 128;  // bytes of a staged weight tile
 constexpr int kMaxStages = 12;
 constexpr int kMaxSplits = 8;
@@ -62,8 +63,8 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-  for (int i = 0; i < kWaitTries; ++i)
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int steps = 0) {
+  for (int64_t i = kWaitTries + int64_t(steps) * kWaitTriesPerStep; i > 0; --i)
     if (mbar_try<CLUSTER>(bar, parity)) return true;
   atomicExch(&g_mx_status, 1);
   return false;
@@ -402,7 +403,7 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   const bool features_whole = w_tile * 128 + 128 <= p.out.features;
   if (warp >= 2) {
     const uint32_t acc = __shfl_sync(0xffffffffu, *tmem_slot, 0) + (uint32_t(warp & 3) * 32 << 16);
-    mbar_wait(done, 0);
+    mbar_wait(done, 0, p.steps);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all of the cluster run
     const int feature = (warp & 3) * 32 + lane;
@@ -440,7 +441,7 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     if (splits > 1 && my_groups > 0) {
       // The other CTAs always send, also after a wait of theirs has run out: wait as long as they may take.
-      for (int i = 0; i < 16 && !mbar_wait<true>(received, 0); ++i) {
+      for (int i = 0; i < 16 && !mbar_wait<true>(received, 0, p.steps); ++i) {
       }
       for (int g = 0; g < my_groups; ++g) {
         const float4* src = exchange + g * 128 + feature;
@@ -627,7 +628,7 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
          unit += (DUAL && (unit & 1) == 0) ? 1 : pairs * kWeights - (DUAL ? 1 : 0)) {
       const int buffer = acc_at.stage;
       const int row0 = int(unit / kWeights / p.pair_tiles) * kPairRows;
-      if (again && !mbar_wait<true>(acc_empty + 8 * buffer, acc_at.parity ^ 1)) break;
+      if (again && !mbar_wait<true>(acc_empty + 8 * buffer, acc_at.parity ^ 1, p.steps)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t acc = tmem + buffer * kPairRows;
       for (int k = 0; k < p.steps; ++k, ring_at.advance(kPairStages)) {
@@ -659,7 +660,7 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
     // every product is done before tensor memory is given back
     if (elect_one()) commit_to_both(drained);
     __syncwarp();
-    mbar_wait(drained, 0);
+    mbar_wait(drained, 0, p.steps);
   } else if (warp >= 2) {
     const uint32_t quarter = uint32_t(warp & 3) * 32, half = uint32_t(warp - 2) / 4;
     constexpr int kCols = kPairRows / 2;  // this warp's columns of a tile
@@ -675,7 +676,7 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
       float gate[DUAL ? kCols : 1];
       if constexpr (DUAL) {
         const int buffer = acc_at.stage;
-        if (!mbar_wait(acc_full + 8 * buffer, acc_at.parity)) break;
+        if (!mbar_wait(acc_full + 8 * buffer, acc_at.parity, 2 * p.steps)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
         for (int c = 0; c < kCols; c += 16) {
@@ -691,7 +692,7 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
         acc_at.advance(2);
       }
       const int buffer = acc_at.stage;
-      if (!mbar_wait(acc_full + 8 * buffer, acc_at.parity)) break;
+      if (!mbar_wait(acc_full + 8 * buffer, acc_at.parity, 2 * p.steps)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
       for (int c = 0; c < kCols; c += 16) {
@@ -809,9 +810,11 @@ int launch_linear(const LinearCall& call, int splits, int smem_limit) {
   const int need = NT * Shape::kWeights + p.stages * int(Shape::kScaleCols);
   p.tmem_cols = need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
   // Shared memory in proportion to the columns: CTAs of these kernels that fit an SM together
-  // never want more than its 512 columns, so none waits for columns while its cluster waits for it.
-  const int smem = std::max(1024 + kTailBytes + p.stages * Shape::kStageBytes + exchange,
-                            int(p.tmem_cols) * (kSmemPerSm / 512) - 1024);
+  // never want more than its 512 columns, so none waits for columns while its cluster waits for it.  A
+  // cluster takes half of an SM at least, which keeps kernels that fill an SM (a library's matrix product on
+  // another stream, which may wait for columns in the same way) from sharing it.
+  const int smem = std::max({1024 + kTailBytes + p.stages * Shape::kStageBytes + exchange,
+                             int(p.tmem_cols) * (kSmemPerSm / 512) - 1024, splits > 1 ? kSmemHalf : 0});
   // instruction descriptor: element types (e4m3 0, e2m1 5), e8m0 scales, N, M = 128
   p.idesc = uint32_t(call.w[0].format == FL_MX_FP8 ? 0 : 5) << 7 | uint32_t(call.x.format == FL_MX_FP8 ? 0 : 5) << 10 |
             uint32_t(NT / 8) << 17 | 1u << 23 | uint32_t(128 / 16) << 24;

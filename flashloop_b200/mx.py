@@ -20,6 +20,7 @@ _raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: a Stream o
 
 FORMATS = {"mxfp8": 0, "mxfp4": 1}
 MAX_NORM_WIDTH = 8192
+MAX_COLUMNS = 2**31 - 256  # of a row: the kernels index a row in 32 bits
 
 
 def _format_code(name: str) -> int:
@@ -54,8 +55,8 @@ class MXTensor:
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, format: str) -> None:
         shape = tuple(int(v) for v in shape)
-        if not shape or min(shape) < 0 or shape[-1] <= 0:
-            raise ValueError("a microscaled tensor needs at least one dimension and a positive last one")
+        if not shape or min(shape) < 0 or not 0 < shape[-1] <= MAX_COLUMNS:
+            raise ValueError(f"a microscaled tensor needs a last dimension of 1 to {MAX_COLUMNS}")
         rows = math.prod(shape[:-1])
         self._code = _format_code(format)
         for t, want, name in ((codes, codes_shape(rows, shape[-1], format), "codes"),
@@ -182,9 +183,9 @@ def mx_quantize(x: torch.Tensor, format: str = "mxfp8") -> MXTensor:
     as NaN."""
 
     _values(x)
-    if x.ndim == 0 or x.shape[-1] == 0:
-        raise ValueError("mx_quantize needs at least one column")
     shape = tuple(x.shape)
+    if not shape or not 0 < shape[-1] <= MAX_COLUMNS:
+        raise ValueError(f"mx_quantize needs a last dimension of 1 to {MAX_COLUMNS} columns")
     cols = shape[-1]
     if x.ndim != 2 or x.stride(1) != 1 or (x.stride(0) < cols and shape[0] > 1):
         x = x.reshape(-1, cols)  # a view where the rows have one stride
@@ -239,7 +240,7 @@ def mx_rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: t
 def _operand(x, weight: MXTensor) -> MXTensor:
     if not isinstance(weight, MXTensor):
         raise TypeError("the weight must be an MXTensor (mx_quantize)")
-    if len(weight.shape) != 2:
+    if len(weight.shape) != 2 or weight.rows > MAX_COLUMNS:
         raise ValueError("the weight must be [out_features, in_features]")
     if isinstance(x, torch.Tensor):
         x = mx_quantize(x, "mxfp8")
@@ -304,6 +305,7 @@ def mx_status(device: torch.device | str = "cuda", *, reset: bool = False) -> in
 
     flag = C.c_int32(-1)
     device = torch.device(device)
+    _require_cuda(device)
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
     with torch.cuda.device(device):

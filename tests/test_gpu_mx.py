@@ -378,6 +378,59 @@ def test_chains_without_waiting():
             assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_inputs_from_another_stream(captured):
+    """What another stream writes before an event is there for the call after it, although the kernel may
+    start before the one in front of it in its own stream has ended."""
+
+    g = _gen("stream")
+    w = fl.mx_quantize(torch.randn(256, 512, generator=g, device="cuda"), "mxfp4")
+    x, fresh = (torch.randn(16, 512, generator=g, device="cuda") for _ in range(2))
+    old, held = x.clone(), fl.mx_quantize(torch.randn(16, 512, generator=g, device="cuda"))
+    want = fl.mx_linear(fl.mx_quantize(fresh), w)
+    side = torch.cuda.Stream()
+
+    def step():
+        main = torch.cuda.current_stream()
+        fl.mx_linear(held, w)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(2_000_000)  # about a millisecond
+            x.copy_(fresh)
+            back = fl.mx_quantize(x)
+        fl.mx_linear(held, w)  # runs meanwhile
+        main.wait_stream(side)
+        return fl.mx_linear(fl.mx_quantize(x), w), fl.mx_linear(back, w)
+
+    run = step
+    if captured:
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        run = lambda: (graph.replay(), outs)[1]
+    for _ in range(3):
+        x.copy_(old)
+        torch.cuda.synchronize()
+        a, b = run()
+        torch.cuda.synchronize()
+        assert torch.equal(a, want) and torch.equal(b, want)
+
+
+def test_long_rows():
+    """More steps of K than a wait has tries, in both kernels."""
+
+    for rows, cols, features in ((2, 400_000, 130), (200 * 192, 140_000, 130)):
+        x = fl.MXTensor(torch.full((rows, -(-cols // 128) * 64), 0x22, dtype=torch.uint8, device="cuda"),
+                        torch.full((-(-rows // 128), -(-cols // 128), 32, 4, 4), 127, dtype=torch.uint8, device="cuda"), (rows, cols), "mxfp4")
+        w = fl.mx_quantize(torch.ones(features, cols, device="cuda", dtype=torch.bfloat16), "mxfp4")
+        y = fl.mx_linear(x, w, out_dtype=torch.float32)  # ones times ones, exact in float32
+        assert bool((y == cols).all())
+        del x, w, y
+    assert mx_status() == 0
+
+
 def test_gradients_are_refused():
     x = torch.randn(2, 64, device="cuda", requires_grad=True)
     with pytest.raises(RuntimeError, match="no gradient"):

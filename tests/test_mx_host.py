@@ -58,6 +58,24 @@ def test_container_checks():
         fl.MXTensor(codes, scales, (), "mxfp8")
 
 
+def test_rows_that_no_index_reaches_are_refused():
+    wide = torch.zeros(1, dtype=torch.bfloat16).expand(2**32 + 64)  # one element of memory
+    with pytest.raises(ValueError, match="columns"):
+        _quantize_as_if_on_a_gpu(wide)
+    with pytest.raises(ValueError, match="last dimension"):
+        fl.MXTensor(torch.zeros(1, 128, dtype=torch.uint8), torch.zeros(1, 1, 32, 4, 4, dtype=torch.uint8), (1, 2**32 + 64), "mxfp8")
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        mx.mx_status("cpu")
+
+
+def _quantize_as_if_on_a_gpu(x):
+    keep, mx._values = mx._values, lambda *tensors: None
+    try:
+        return mx.mx_quantize(x)
+    finally:
+        mx._values = keep
+
+
 def test_refusals_before_the_gpu():
     x = torch.zeros(2, 64)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
