@@ -941,13 +941,16 @@ const Device& device_limits(int device) {
 }
 
 // How a call is cut, by its tiles of 128 features by NT rows and its steps of K:
-// - up to 32 rows, CTAs take half of an SM's shared memory, so that two fit an SM and the next kernel's can set up beside
-//   the last ones of this; K is split while that gives at most three CTAs to two SMs and three steps to a CTA
+// - up to 32 rows (16 of a gated product, whose stages are twice as large), CTAs take half of an SM's shared memory, so
+//   that two fit an SM and the next kernel's can set up beside the last ones of this; K is split while that gives at most three CTAs to two SMs and three steps to a CTA
 //   (16 rows, mxfp4, weights not in L2; 2048 -> 6144: split two ways with all of the shared memory 4.7 us, two ways
 //   with half 4.8, three 4.4, four 4.1, five 4.5; 2048 -> 2048: four 3.4, six 3.3, eight 3.4; 5632 -> 2048: four
 //   5.2, six 4.5, eight 4.3; gated 2048 -> 5632: two with all 7.0, three with all 6.7, five with half 6.5);
-// - with more rows the exchange of the sums weighs more: two CTAs to three SMs, each taking all of its shared memory
-//   (64 rows, 2048 -> 6144: two ways 6.5 us, three 7.9);
+// - with more rows the exchange of the sums takes as long as some rows / 4 steps: K is split three ways or more where
+//   K has as many and that leaves a third of the SMs idle (none up to 32 rows), by CTAs that take all of an SM's shared memory
+//   (64 rows, 2048 -> 6144: whole 6.0 us, two ways 6.6; 2048 -> 2048: whole 5.7, two ways 6.0, three 5.1, six 4.9;
+//   128 rows, 2048 -> 2048: whole 7.1, two ways 8.3, four 7.5; 5632 -> 2048: whole 12.8, two ways 12.0, six 9.2;
+//   gated 64 rows, 2048 -> 5632: whole 10.4, two ways 11.8);
 // - never more than run at once: a cluster that waits for another to end doubles the call (2048 -> 6144
 //   split three ways with all of the shared memory: 7.8 us);
 // - pairs of CTAs once tiles of 128 rows (64 of a gated product) no longer run at once (2048 -> 6144: 384 rows 8.5 us
@@ -959,19 +962,21 @@ int choose_linear(const LinearCall& call) {
   const int sms = device.sms;
   const int steps = int(mx_steps(call.cols));
   const int64_t w_tiles = (call.features + 127) / 128;
-  auto splits_for = [&](int nt) {
-    const bool half = nt <= 32;
-    const int64_t tiles = (call.rows + nt - 1) / nt * w_tiles;
+  auto run = [&](auto nt, bool half) {
+    constexpr int kRows = decltype(nt)::value;
+    const int64_t tiles = (call.rows + kRows - 1) / kRows * w_tiles;
+    const int64_t most = half ? sms * 3 / 2 : kRows <= 32 ? sms : sms * 2 / 3;
     int splits = std::max(1, std::min(kMaxSplits, (steps + 2) / 3));
-    while (splits > 1 && (tiles * splits > (half ? sms * 3 / 2 : sms * 2 / 3) || tiles > device.clusters[half][splits])) --splits;
-    return splits;
+    while (splits > 1 && (tiles * splits > most || tiles > device.clusters[half][splits])) --splits;
+    if (!half && (splits < 3 || steps < std::min<int64_t>(call.rows, kRows) / 4)) splits = 1;
+    return launch_linear<KIND, kRows, DUAL>(call, splits, half ? kSmemHalf : kSmemLimit);
   };
-  if (call.rows <= 16) return launch_linear<KIND, 16, DUAL>(call, splits_for(16), kSmemHalf);
-  if (call.rows <= 32) return launch_linear<KIND, 32, DUAL>(call, splits_for(32), kSmemHalf);
-  if (call.rows <= 64) return launch_linear<KIND, 64, DUAL>(call, splits_for(64), kSmemLimit);
+  if (call.rows <= 16) return run(std::integral_constant<int, 16>{}, true);
+  if (call.rows <= 32) return run(std::integral_constant<int, 32>{}, !DUAL);
+  if (call.rows <= 64) return run(std::integral_constant<int, 64>{}, false);
   constexpr int kTile = DUAL ? 64 : 128;
   if ((call.rows + kTile - 1) / kTile * w_tiles > sms) return launch_pairs<KIND, DUAL>(call, sms);
-  return launch_linear<KIND, kTile, DUAL>(call, splits_for(kTile), kSmemLimit);
+  return run(std::integral_constant<int, kTile>{}, false);
 }
 
 template <bool DUAL>
