@@ -172,17 +172,19 @@ struct Output {
 
 // Stores N rows of this thread's feature n, from row m on, of which `count` exist.  The 32 lanes of a
 // warp hold 32 consecutive features, which are one block of a microscaled result; whole warps call it.
-// WHOLE: all N rows and the feature exist.  That path has no branches: the epilogue of many rows is
-// bound by the instructions of its eight warps.
+// WHOLE: all N rows exist.  That path has one branch at most: the epilogue of many rows is bound by the
+// instructions of its eight warps.
 template <int KIND, bool WHOLE, int N>
 __device__ __forceinline__ void emit_rows(const Output& o, int64_t m, int n, const float (&v)[N], int count) {
-  const bool live = WHOLE || n < o.features;
+  const bool live = n < o.features;
   if constexpr (KIND <= kOutF32) {
     using T = std::conditional_t<KIND == kOutBf16, __nv_bfloat16, std::conditional_t<KIND == kOutF16, __half, float>>;
     T* dst = static_cast<T*>(o.data) + m * o.features + n;
+    if (live) {
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (WHOLE || (live && j < count)) dst[int64_t(j) * o.features] = round_to<T>(v[j]);
+      for (int j = 0; j < N; ++j)
+        if (WHOLE || j < count) dst[int64_t(j) * o.features] = round_to<T>(v[j]);
+    }
   } else {
     // m is a multiple of N, a divisor of 32, so that the scales of these rows lie sixteen bytes apart
     static_assert(N % 4 == 0 && 32 % N == 0, "rows of one scale group, four to a word");
@@ -400,7 +402,6 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   __syncwarp();
 
   const int n = w_tile * 128 + (warp & 3) * 32 + lane;
-  const bool features_whole = w_tile * 128 + 128 <= p.out.features;
   if (warp >= 2) {
     const uint32_t acc = __shfl_sync(0xffffffffu, *tmem_slot, 0) + (uint32_t(warp & 3) * 32 << 16);
     mbar_wait(done, 0, p.steps);
@@ -431,7 +432,7 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           v[j] = DUAL ? gated(__uint_as_float(a[j]), __uint_as_float(b[j])) : __uint_as_float(a[j]);
-        if (features_whole && c + 16 <= cols) {
+        if (c + 16 <= cols) {
           emit_rows<KIND, true>(p.out, row0 + c, n, v, 16);
         } else {
           emit_rows<KIND, false>(p.out, row0 + c, n, v, cols - c);
@@ -462,7 +463,7 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
           for (int j = 0; j < 4; ++j) v[j] = gated(v[j], u[j]);
         }
         const int c = (rank * groups + g) * 4;
-        if (features_whole && c + 4 <= cols) {
+        if (c + 4 <= cols) {
           emit_rows<KIND, true>(p.out, row0 + c, n, v, 4);
         } else {
           emit_rows<KIND, false>(p.out, row0 + c, n, v, cols - c);
@@ -672,7 +673,7 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
       const int n = n0 + int(quarter) + lane;
       const int64_t m0 = tile / p.pair_tiles * kPairRows + half * kCols;
       const int cols = n0 < p.out.features ? int(max(int64_t(0), min(int64_t(kCols), p.rows - m0))) : 0;
-      const bool whole = cols == kCols && n0 + 128 <= p.out.features;
+      const bool whole = cols == kCols;
       float gate[DUAL ? kCols : 1];
       if constexpr (DUAL) {
         const int buffer = acc_at.stage;
@@ -946,11 +947,11 @@ const Device& device_limits(int device) {
 //   (16 rows, mxfp4, weights not in L2; 2048 -> 6144: split two ways with all of the shared memory 4.7 us, two ways
 //   with half 4.8, three 4.4, four 4.1, five 4.5; 2048 -> 2048: four 3.4, six 3.3, eight 3.4; 5632 -> 2048: four
 //   5.2, six 4.5, eight 4.3; gated 2048 -> 5632: two with all 7.0, three with all 6.7, five with half 6.5);
-// - with more rows the exchange of the sums takes as long as some rows / 4 steps: K is split three ways or more where
-//   K has as many and that leaves a third of the SMs idle (none up to 32 rows), by CTAs that take all of an SM's shared memory
-//   (64 rows, 2048 -> 6144: whole 6.0 us, two ways 6.6; 2048 -> 2048: whole 5.7, two ways 6.0, three 5.1, six 4.9;
-//   128 rows, 2048 -> 2048: whole 7.1, two ways 8.3, four 7.5; 5632 -> 2048: whole 12.8, two ways 12.0, six 9.2;
-//   gated 64 rows, 2048 -> 5632: whole 10.4, two ways 11.8);
+// - with more rows CTAs take all of an SM's shared memory, and K is split while that leaves a third of the SMs idle (none
+//   up to 32 rows).  The exchange of the sums takes longer the more rows there are, so that it has to save some
+//   rows / 8 steps, of which a two-way split saves only half (warm weights; 2048 -> 2048: 64 rows whole 5.7 us, six
+//   ways 4.8, 96 rows 6.6 and 5.9, 128 rows 7.0 and 7.7, 128 rows of 4096 -> 2048 10.2 and 8.5; 2048 -> 6144: 40 rows
+//   whole 5.9, two ways 5.5, 64 rows 5.8 and 6.3; gated 1000 -> 2048: 40 rows whole 6.9, five ways 5.3);
 // - never more than run at once: a cluster that waits for another to end doubles the call (2048 -> 6144
 //   split three ways with all of the shared memory: 7.8 us);
 // - pairs of CTAs once tiles of 128 rows (64 of a gated product) no longer run at once (2048 -> 6144: 384 rows 8.5 us
@@ -968,7 +969,7 @@ int choose_linear(const LinearCall& call) {
     const int64_t most = half ? sms * 3 / 2 : kRows <= 32 ? sms : sms * 2 / 3;
     int splits = std::max(1, std::min(kMaxSplits, (steps + 2) / 3));
     while (splits > 1 && (tiles * splits > most || tiles > device.clusters[half][splits])) --splits;
-    if (!half && (splits < 3 || steps < std::min<int64_t>(call.rows, kRows) / 4)) splits = 1;
+    if (!half && steps * (splits == 2 ? 3 : 8) <= std::min<int64_t>(call.rows, kRows)) splits = 1;
     return launch_linear<KIND, kRows, DUAL>(call, splits, half ? kSmemHalf : kSmemLimit);
   };
   if (call.rows <= 16) return run(std::integral_constant<int, 16>{}, true);
