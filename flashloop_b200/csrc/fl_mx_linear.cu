@@ -11,8 +11,12 @@
 // go on to tensor memory with tcgen05.cp.  With few output tiles K is split over the CTAs of a cluster,
 // which add their accumulators through distributed shared memory in rank order.
 //
-// Warp 0 issues the copies, warp 1 the matrix instructions, warps 2-5 run the epilogue.  Every wait
-// is bounded: a wait that runs out raises a status word and the kernel runs to its end.
+// Every wait on a copy or another CTA's sums is bounded: one that runs out raises a status word and the kernel runs to its
+// end.
+//
+// may_start_next() comes after a CTA has its tensor memory, so that a kernel let in early never holds columns
+// that this one still needs.  The other way round, a kernel that waits for the one before it holds few columns (few
+// rows: at most 256 to the half of an SM's shared memory) or allocates after the wait (many rows).
 #include <cuda.h>
 
 #include <algorithm>
@@ -159,7 +163,7 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
 
 // silu(g) * u.  The exponential and the quotient are the hardware's approximations, a few units in the last place of
 // float32: far below the rounding of the operands, and the exact forms cost the epilogue more than the
-// products take (gated 16384 x 2048 -> 5632: 421 us with expf and a rounded division, 265 us with these and emit16).
+// products take (gated 16384 x 2048 -> 5632: 421 us with expf and a rounded division, 265 us with these and without branches in the stores).
 __device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
 
 // Where a product goes.
@@ -539,6 +543,10 @@ __device__ __forceinline__ void commit_to_both(uint32_t bar) {
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
       ::"r"(bar), "h"(uint16_t(3)) : "memory");
 }
+// ... and on that of this CTA alone: the other one may be gone when it comes.
+__device__ __forceinline__ void commit_here(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
@@ -557,6 +565,7 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
   const int64_t pairs = gridDim.x / 2, pair = blockIdx.x / 2;
   constexpr int kWeights = DUAL ? 2 : 1;
 
+  wait_for_inputs();
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(512u)
                  : "memory");
@@ -577,7 +586,6 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   cluster_sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  wait_for_inputs();
   may_start_next();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const uint32_t tmem_scales = tmem + 2 * kPairRows;
@@ -617,9 +625,9 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
     }
     // leave only when every copy of the pair has landed: the stages of this round, then those of the last
     if (rank == 0) {
-      for (int s = 0; ok && s < kPairStages; ++s) {
+      for (int s = 0; s < kPairStages; ++s) {
         const bool this_round = s < ring_at.stage;
-        if (this_round || again) ok = mbar_wait(full + 8 * s, this_round ? ring_at.parity : ring_at.parity ^ 1);
+        if (this_round || again) mbar_wait(full + 8 * s, this_round ? ring_at.parity : ring_at.parity ^ 1);
       }
     }
   } else if (warp == 1 && rank == 0) {
@@ -659,7 +667,7 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
       again |= acc_at.stage == 0;
     }
     // every product is done before tensor memory is given back
-    if (elect_one()) commit_to_both(drained);
+    if (elect_one()) commit_here(drained);
     __syncwarp();
     mbar_wait(drained, 0, p.steps);
   } else if (warp >= 2) {
@@ -810,12 +818,12 @@ int launch_linear(const LinearCall& call, int splits, int smem_limit) {
   p.stages = std::min({kMaxStages, room, (steps + splits - 1) / splits});
   const int need = NT * Shape::kWeights + p.stages * int(Shape::kScaleCols);
   p.tmem_cols = need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
-  // Shared memory in proportion to the columns: CTAs of these kernels that fit an SM together
-  // never want more than its 512 columns, so none waits for columns while its cluster waits for it.  A
-  // cluster takes half of an SM at least, which keeps kernels that fill an SM (a library's matrix product on
-  // another stream, which may wait for columns in the same way) from sharing it.
+  // Shared memory in proportion to the columns: CTAs of these kernels that fit an SM together never want more
+  // than its 512 columns, so none waits for columns while its cluster waits for it.  Half of an SM's at least, which
+  // keeps kernels that fill an SM (a library's matrix product before this one or on another stream, which may wait
+  // for columns in the same way) from sharing it.
   const int smem = std::max({1024 + kTailBytes + p.stages * Shape::kStageBytes + exchange,
-                             int(p.tmem_cols) * (kSmemPerSm / 512) - 1024, splits > 1 ? kSmemHalf : 0});
+                             int(p.tmem_cols) * (kSmemPerSm / 512) - 1024, kSmemHalf});
   // instruction descriptor: element types (e4m3 0, e2m1 5), e8m0 scales, N, M = 128
   p.idesc = uint32_t(call.w[0].format == FL_MX_FP8 ? 0 : 5) << 7 | uint32_t(call.x.format == FL_MX_FP8 ? 0 : 5) << 10 |
             uint32_t(NT / 8) << 17 | 1u << 23 | uint32_t(128 / 16) << 24;
