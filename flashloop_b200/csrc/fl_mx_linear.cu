@@ -1,7 +1,7 @@
 // Projections of microscaled operands on the tensor cores:
 //   y[m][n] = sum over blocks b of 2^(sx[m][b] + sw[n][b]) * sum over k in b of x[m][k] * w[n][k]
 // with float32 accumulation, plain or as silu(gate) * up of two weights.  Both operands may be e4m3 or
-// e2m1 (tcgen05.mma kind::mxf8f6f4 with block scales takes any pairing).
+// e2m1 (tcgen05.mma kind::mxf8f6f4 with block scales takes any pairing; many rows of e2m1 by e2m1 use kind::mxf4).
 //
 // The weight is the 128-row operand of the instruction and the rows of x are its columns, so one
 // kernel serves one row of x as well as thousands: the accumulator is [128 features][NT rows of x] in
@@ -494,19 +494,30 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 //
 // silu(gate) * up: the gate tile and the up tile of the same features are two units one after the
 // other; the epilogue moves the gate accumulator to registers while the up products run.
+//
+// PACKED: both operands are e2m1.  They stay packed in shared memory, 256 elements to a stage, and go through
+// kind::mxf4, 64 elements an instruction at twice the rate (32768 x 5632 -> 2048: 139 us = 5440 TFLOP/s against 257 us
+// with x in mxfp8; gated 16384 x 2048 -> 5632: 210 against 270 us, where the epilogue is the longer part).
 
 constexpr int kPairThreads = 320;  // copies, matrix instructions, eight epilogue warps
 // NT: rows of x per tile.  A multiple of 64, as the scales of x start at an even column of tensor memory.
 constexpr int kPairRows = 192;
-constexpr int kPairStages = 7;
 constexpr int kPairXTiles = 2;  // scale tiles that 192 rows starting at a multiple of 64 touch
 constexpr int kPairXBytes = kPairRows / 2 * 128;
 constexpr int kPairScalesAt = kTileW + kPairXBytes;
-constexpr int kPairStageBytes = (kPairScalesAt + (1 + kPairXTiles) * kMxTileBytes + 1023) / 1024 * 1024;
-constexpr uint32_t kPairScaleCols = 4 * (1 + kPairXTiles);
+
+template <bool PACKED>
+struct Pair {
+  static constexpr int kSteps = PACKED ? 2 : 1;  // of K in a stage
+  // scales of a stage, in shared memory and in tensor memory: those of the weight step by step, then those of x
+  static constexpr int kScaleTiles = kSteps * (1 + kPairXTiles);
+  static constexpr uint32_t kScaleCols = 4 * kScaleTiles;
+  static constexpr int kStageBytes = (kPairScalesAt + kScaleTiles * kMxTileBytes + 1023) / 1024 * 1024;
+  static constexpr int kStages = PACKED ? 5 : 7;
+  static_assert(2 * kPairRows + kStages * kScaleCols <= 512, "tensor memory columns");
+  static_assert(1024 + kStages * kStageBytes + kTailBytes <= kSmemLimit, "shared memory");
+};
 static_assert(kPairXBytes % 1024 == 0, "tiles need 1024-byte alignment");
-static_assert(2 * kPairRows + kPairStages * kPairScaleCols <= 512, "tensor memory columns");
-static_assert(1024 + kPairStages * kPairStageBytes + kTailBytes <= kSmemLimit, "shared memory");
 
 struct PairMaps {
   CUtensorMap x, x_scales, w[2], w_scales[2];
@@ -518,7 +529,7 @@ struct PairParams {
   int steps;
   int pair_tiles;    // of 256 features
   int64_t units;     // tiles times weights
-  uint32_t step_bytes;  // that the copies of one step report, both CTAs
+  uint32_t stage_bytes;  // that the copies of one stage report, both CTAs
   uint32_t idesc;
 };
 
@@ -530,12 +541,20 @@ __device__ __forceinline__ void copy_tile_pair(uint32_t dst, const CUtensorMap* 
 __device__ __forceinline__ void scales_to_tmem_pair(uint32_t taddr, uint32_t smem) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(scale_desc(smem)) : "memory");
 }
+template <bool PACKED>
 __device__ __forceinline__ void mma_mx_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                             uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+  if constexpr (PACKED) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+  }
 }
 // Arrives on the barrier at this offset in both CTAs once every matrix instruction issued so far is done.
 __device__ __forceinline__ void commit_to_both(uint32_t bar) {
@@ -551,15 +570,17 @@ __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
-template <int KIND, bool DUAL>
+template <int KIND, bool DUAL, bool PACKED>
 __global__ void __launch_bounds__(kPairThreads)
 mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
+  using Shape = Pair<PACKED>;
+  constexpr int kStages = Shape::kStages, kStageBytes = Shape::kStageBytes, kSteps = Shape::kSteps;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* smem = raw_smem + (1024 - (smem_addr(raw_smem) & 1023)) % 1024;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kPairStages * kPairStageBytes);
-  const uint32_t ring = smem_addr(smem), full = smem_addr(bars), empty = full + 8 * kPairStages,
-                 acc_full = empty + 8 * kPairStages, acc_empty = acc_full + 16, drained = acc_empty + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kPairStages + 5);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
+  const uint32_t ring = smem_addr(smem), full = smem_addr(bars), empty = full + 8 * kStages,
+                 acc_full = empty + 8 * kStages, acc_empty = acc_full + 16, drained = acc_empty + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 5);
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) / 32, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int64_t pairs = gridDim.x / 2, pair = blockIdx.x / 2;
@@ -572,7 +593,7 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
   if (threadIdx.x == 32) {
-    for (int s = 0; s < kPairStages; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(full + 8 * s, 1);
       mbar_init(empty + 8 * s, 1);
     }
@@ -601,31 +622,37 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
       const int which = int(unit % kWeights);
       const int w_tile = int(tile % p.pair_tiles) * 2 + int(rank);
       const int row0 = int(tile / p.pair_tiles) * kPairRows;
-      for (int k = 0; k < p.steps; ++k) {
+      for (int k = 0; k < p.steps; k += kSteps) {
         const int s = ring_at.stage;
         if (again && !mbar_wait(empty + 8 * s, ring_at.parity ^ 1)) {
           ok = false;
           break;
         }
-        const uint32_t at = ring + s * kPairStageBytes, bar = leader_full + 8 * s;
+        const uint32_t at = ring + s * kStageBytes, bar = leader_full + 8 * s;
         if (elect_one()) {
-          if (rank == 0) mbar_expect(full + 8 * s, p.step_bytes);
-          copy_tile_pair(at, &maps.w[which], k * kMxStep, w_tile * 128, bar);
-          copy_tile_pair(at + kTileW, &maps.x, k * kMxStep, row0 + int(rank) * (kPairRows / 2), bar);
-          copy_tile_pair(at + kPairScalesAt, &maps.w_scales[which], 0, w_tile * p.steps + k, bar);
+          if (rank == 0) mbar_expect(full + 8 * s, p.stage_bytes);
+          // packed codes are copied as bytes, two elements each
+          const int at_k = PACKED ? k * (kMxStep / 2) : k * kMxStep;
+          copy_tile_pair(at, &maps.w[which], at_k, w_tile * 128, bar);
+          copy_tile_pair(at + kTileW, &maps.x, at_k, row0 + int(rank) * (kPairRows / 2), bar);
+          uint32_t scales = at + kPairScalesAt;
 #pragma unroll
-          for (int i = 0; i < kPairXTiles; ++i)
-            copy_tile_pair(at + kPairScalesAt + (1 + i) * kMxTileBytes, &maps.x_scales, 0,
-                           (row0 / kMxTileRows + i) * p.steps + k, bar);
+          for (int j = 0; j < kSteps; ++j, scales += kMxTileBytes)
+            copy_tile_pair(scales, &maps.w_scales[which], 0, w_tile * p.steps + k + j, bar);
+#pragma unroll
+          for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+            for (int i = 0; i < kPairXTiles; ++i, scales += kMxTileBytes)
+              copy_tile_pair(scales, &maps.x_scales, 0, (row0 / kMxTileRows + i) * p.steps + k + j, bar);
         }
         __syncwarp();
-        ring_at.advance(kPairStages);
+        ring_at.advance(kStages);
         again |= ring_at.stage == 0;
       }
     }
     // leave only when every copy of the pair has landed: the stages of this round, then those of the last
     if (rank == 0) {
-      for (int s = 0; s < kPairStages; ++s) {
+      for (int s = 0; s < kStages; ++s) {
         const bool this_round = s < ring_at.stage;
         if (this_round || again) mbar_wait(full + 8 * s, this_round ? ring_at.parity : ring_at.parity ^ 1);
       }
@@ -640,23 +667,28 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
       if (again && !mbar_wait<true>(acc_empty + 8 * buffer, acc_at.parity ^ 1, p.steps)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t acc = tmem + buffer * kPairRows;
-      for (int k = 0; k < p.steps; ++k, ring_at.advance(kPairStages)) {
+      for (int k = 0; k < p.steps; k += kSteps, ring_at.advance(kStages)) {
         const int s = ring_at.stage;
         if (!mbar_wait(full + 8 * s, ring_at.parity)) {
           ok = false;
           break;
         }
-        const uint32_t at = ring + s * kPairStageBytes, scales = at + kPairScalesAt;
-        const uint32_t sf = tmem_scales + uint32_t(s) * kPairScaleCols;
+        const uint32_t at = ring + s * kStageBytes, scales = at + kPairScalesAt;
+        const uint32_t sf = tmem_scales + uint32_t(s) * Shape::kScaleCols;
         const uint64_t w_desc = tile_desc(at), x_desc = tile_desc(at + kTileW);
-        const uint32_t sfb = sf + 4 + (row0 % kMxTileRows) / 32;
+        const uint32_t sfb = sf + 4 * kSteps + (row0 % kMxTileRows) / 32;
         if (elect_one()) {
 #pragma unroll
-          for (int t = 0; t < 1 + kPairXTiles; ++t) scales_to_tmem_pair(sf + 4 * t, scales + t * kMxTileBytes);
+          for (int t = 0; t < Shape::kScaleTiles; ++t) scales_to_tmem_pair(sf + 4 * t, scales + t * kMxTileBytes);
+          // Four instructions of 32 bytes along the swizzled row: a block each, or packed two blocks, of which a step
+          // has two pairs.  What lies past the last step of a stage is not multiplied (its scales are another tile's).
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
-            mma_mx_pair(acc, w_desc + 2 * b, x_desc + 2 * b, p.idesc | uint32_t(b) << 29 | uint32_t(b) << 4, sf, sfb,
-                        k > 0 || b > 0);
+          for (int b = 0; b < 4; ++b) {
+            const uint32_t step = PACKED ? b / 2 : 0, block = PACKED ? b % 2 * 2 : b;
+            if (!PACKED || b < 2 || k + 1 < p.steps)
+              mma_mx_pair<PACKED>(acc, w_desc + 2 * b, x_desc + 2 * b, p.idesc | block << 29 | block << 4, sf + 4 * step,
+                                  sfb + 4 * kPairXTiles * step, k > 0 || b > 0);
+          }
           commit_to_both(empty + 8 * s);
         }
         __syncwarp();
@@ -754,17 +786,18 @@ EncodeTiled encode_tiled() {
   return fn;
 }
 
-// Codes [rows][steps * 128] as boxes of 128 elements by box_rows rows in the 128-byte swizzle; rows past
-// the last read as zero.
-bool make_map(CUtensorMap* map, const void* codes, int format, int64_t rows, int64_t steps, int box_rows) {
+// Codes [rows][steps * 128] as boxes of 128 elements by box_rows rows in the 128-byte swizzle, or, packed, of 128
+// bytes of e2m1; rows past the last and bytes past the end of a row read as zero.
+bool make_map(CUtensorMap* map, const void* codes, int format, int64_t rows, int64_t steps, int box_rows,
+              bool packed = false) {
   const EncodeTiled encode = encode_tiled();
   if (encode == nullptr) return false;
   const bool fp8 = format == FL_MX_FP8;
-  const cuuint64_t dims[2] = {cuuint64_t(steps * kMxStep), cuuint64_t(rows)};
+  const cuuint64_t dims[2] = {cuuint64_t(steps * (packed ? kMxStep / 2 : kMxStep)), cuuint64_t(rows)};
   const cuuint64_t strides[1] = {cuuint64_t(steps * (fp8 ? kMxStep : kMxStep / 2))};
   const cuuint32_t box[2] = {kMxStep, cuuint32_t(box_rows)};
   const cuuint32_t unit[2] = {1, 1};
-  return encode(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2,
+  return encode(map, fp8 || packed ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2,
                 const_cast<void*>(codes), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -864,8 +897,9 @@ bool make_scale_map(CUtensorMap* map, const void* scales, int64_t rows, int64_t 
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int KIND, bool DUAL>
+template <int KIND, bool DUAL, bool PACKED>
 int launch_pairs(const LinearCall& call, int sms) {
+  using Shape = Pair<PACKED>;
   const int steps = int(mx_steps(call.cols));
   PairMaps maps;
   PairParams p;
@@ -875,15 +909,16 @@ int launch_pairs(const LinearCall& call, int sms) {
   p.pair_tiles = (call.features + 255) / 256;
   const int64_t tiles = (call.rows + kPairRows - 1) / kPairRows * p.pair_tiles;
   p.units = tiles * (DUAL ? 2 : 1);
-  p.step_bytes = 2 * uint32_t((kTileW >> (call.w[0].format == FL_MX_FP8 ? 0 : 1)) +
-                              (kPairXBytes >> (call.x.format == FL_MX_FP8 ? 0 : 1)) + (1 + kPairXTiles) * kMxTileBytes);
-  p.idesc = uint32_t(call.w[0].format == FL_MX_FP8 ? 0 : 5) << 7 | uint32_t(call.x.format == FL_MX_FP8 ? 0 : 5) << 10 |
-            uint32_t(kPairRows / 8) << 17 | 1u << 23 | uint32_t(256 / 16) << 24;
-  bool ok = make_map(&maps.x, call.x.codes, call.x.format, call.rows, steps, kPairRows / 2) &&
+  const bool w_spread = !PACKED && call.w[0].format == FL_MX_FP4, x_spread = !PACKED && call.x.format == FL_MX_FP4;
+  p.stage_bytes = 2 * uint32_t((kTileW >> int(w_spread)) + (kPairXBytes >> int(x_spread)) + Shape::kScaleTiles * kMxTileBytes);
+  // element types as in launch_linear, or e2m1 of kind::mxf4 (1)
+  const uint32_t w_type = PACKED ? 1 : w_spread ? 5 : 0, x_type = PACKED ? 1 : x_spread ? 5 : 0;
+  p.idesc = w_type << 7 | x_type << 10 | uint32_t(kPairRows / 8) << 17 | 1u << 23 | uint32_t(256 / 16) << 24;
+  bool ok = make_map(&maps.x, call.x.codes, call.x.format, call.rows, steps, kPairRows / 2, PACKED) &&
             make_scale_map(&maps.x_scales, call.x.scales, call.rows, steps);
   for (int i = 0; i < (DUAL ? 2 : 1); ++i) {
     const Operand& w = call.w[i];
-    ok = ok && make_map(&maps.w[i], w.codes, w.format, call.features, steps, 128) &&
+    ok = ok && make_map(&maps.w[i], w.codes, w.format, call.features, steps, 128, PACKED) &&
          make_scale_map(&maps.w_scales[i], w.scales, call.features, steps);
   }
   if (!DUAL) {
@@ -894,7 +929,7 @@ int launch_pairs(const LinearCall& call, int sms) {
   FL_REQUIRE(int64_t(p.out.w_tiles + 2) * steps < (int64_t(1) << 31) &&
                  (call.rows / kMxTileRows + kPairXTiles + 1) * steps < (int64_t(1) << 31),
              "%s: too many elements", call.who);
-  auto kernel = mx_linear_pair_kernel<KIND, DUAL>;
+  auto kernel = mx_linear_pair_kernel<KIND, DUAL, PACKED>;
   static std::atomic<bool> allowed[kMaxDevices];
   cudaError_t err = allow_shared_memory(kernel, allowed, call.device);
   // all of an SM's shared memory, as it takes all of its tensor memory (see above)
@@ -984,7 +1019,10 @@ int choose_linear(const LinearCall& call) {
   if (call.rows <= 32) return run(std::integral_constant<int, 32>{}, !DUAL);
   if (call.rows <= 64) return run(std::integral_constant<int, 64>{}, false);
   constexpr int kTile = DUAL ? 64 : 128;
-  if ((call.rows + kTile - 1) / kTile * w_tiles > sms) return launch_pairs<KIND, DUAL>(call, sms);
+  if ((call.rows + kTile - 1) / kTile * w_tiles > sms) {
+    const bool packed = call.x.format == FL_MX_FP4 && call.w[0].format == FL_MX_FP4;
+    return packed ? launch_pairs<KIND, DUAL, true>(call, sms) : launch_pairs<KIND, DUAL, false>(call, sms);
+  }
   return run(std::integral_constant<int, kTile>{}, false);
 }
 

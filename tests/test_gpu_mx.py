@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import flashloop_b200 as fl
-from flashloop_b200.mx import mx_status
+from flashloop_b200.mx import codes_shape, mx_status, scales_shape
 from tests import mx_reference as ref
 
 pytestmark = pytest.mark.gpu
@@ -213,7 +213,7 @@ def test_linear(rows, cols, features, x_format, w_format):
 
 
 @pytest.mark.parametrize("rows,cols,features", SIZES)
-@pytest.mark.parametrize("x_format,w_format", [("mxfp8", "mxfp4"), ("mxfp4", "mxfp8")])
+@pytest.mark.parametrize("x_format,w_format", [("mxfp8", "mxfp4"), ("mxfp4", "mxfp8"), ("mxfp4", "mxfp4")])
 def test_linear_swiglu(rows, cols, features, x_format, w_format):
     x, (gate, up) = _operands(rows, cols, features, x_format, w_format, weights=2)
     g, g_magnitude = _product64(x, gate)
@@ -248,13 +248,14 @@ def test_linear_quantises_a_plain_tensor_and_keeps_leading_dimensions():
     assert fl.mx_linear_swiglu(x[:0], w, w, out_format="mxfp8").shape == (0, 3, 70)
 
 
-@pytest.mark.parametrize("rows", [5, 200])
-def test_linear_blocks_that_are_not_finite(rows):
+@pytest.mark.parametrize("rows", [5, 200, 19500])
+@pytest.mark.parametrize("x_format", ["mxfp8", "mxfp4"])
+def test_linear_blocks_that_are_not_finite(rows, x_format):
     x = torch.randn(rows, 300, generator=_gen("nan", rows), device="cuda")
     w = torch.randn(140, 300, generator=_gen("nan", rows + 1), device="cuda")
     x[3, 100] = float("inf")
     w[131, 299] = float("nan")
-    y = fl.mx_linear(x, fl.mx_quantize(w, "mxfp4"))
+    y = fl.mx_linear(fl.mx_quantize(x, x_format), fl.mx_quantize(w, "mxfp4"))
     bad = torch.zeros(rows, 140, dtype=torch.bool, device="cuda")
     bad[3], bad[:, 131] = True, True
     assert torch.equal(torch.isnan(y), bad)
@@ -263,11 +264,12 @@ def test_linear_blocks_that_are_not_finite(rows):
 def test_linear_of_extreme_scales():
     """Scales near both ends of their range whose products are ordinary, and zero rows."""
 
-    x = torch.randn(20, 256, generator=_gen("extreme"), device="cuda")
-    w = torch.randn(30, 256, generator=_gen("extreme", 1), device="cuda")
-    small, large = fl.mx_quantize(x * 2.0 ** -100, "mxfp8"), fl.mx_quantize(w * 2.0 ** 110, "mxfp4")
-    plain = fl.mx_linear(fl.mx_quantize(x, "mxfp8"), fl.mx_quantize(w, "mxfp4"), out_dtype=torch.float32)
-    assert torch.equal(fl.mx_linear(small, large, out_dtype=torch.float32), plain * 2.0 ** 10)
+    for rows, x_format in ((20, "mxfp8"), (20, "mxfp4"), (19500, "mxfp8"), (19500, "mxfp4")):
+        x = torch.randn(rows, 256, generator=_gen("extreme"), device="cuda")
+        w = torch.randn(30, 256, generator=_gen("extreme", 1), device="cuda")
+        small, large = fl.mx_quantize(x * 2.0 ** -100, x_format), fl.mx_quantize(w * 2.0 ** 110, "mxfp4")
+        plain = fl.mx_linear(fl.mx_quantize(x, x_format), fl.mx_quantize(w, "mxfp4"), out_dtype=torch.float32)
+        assert torch.equal(fl.mx_linear(small, large, out_dtype=torch.float32), plain * 2.0 ** 10)
     zero = fl.mx_linear(torch.zeros_like(x), fl.mx_quantize(w, "mxfp4"))
     assert not zero.any()
 
@@ -421,9 +423,10 @@ def test_inputs_from_another_stream(captured):
 def test_long_rows():
     """More steps of K than a wait has tries, in both kernels."""
 
-    for rows, cols, features in ((2, 400_000, 130), (200 * 192, 140_000, 130)):
-        x = fl.MXTensor(torch.full((rows, -(-cols // 128) * 64), 0x22, dtype=torch.uint8, device="cuda"),
-                        torch.full((-(-rows // 128), -(-cols // 128), 32, 4, 4), 127, dtype=torch.uint8, device="cuda"), (rows, cols), "mxfp4")
+    for rows, cols, features, x_format, one in ((2, 400_000, 130, "mxfp4", 0x22), (200 * 192, 140_000, 130, "mxfp8", 0x38),
+                                                (200 * 192, 140_000, 130, "mxfp4", 0x22)):
+        x = fl.MXTensor(torch.full(codes_shape(rows, cols, x_format), one, dtype=torch.uint8, device="cuda"),
+                        torch.full(scales_shape(rows, cols), 127, dtype=torch.uint8, device="cuda"), (rows, cols), x_format)
         w = fl.mx_quantize(torch.ones(features, cols, device="cuda", dtype=torch.bfloat16), "mxfp4")
         y = fl.mx_linear(x, w, out_dtype=torch.float32)  # ones times ones, exact in float32
         assert bool((y == cols).all())
