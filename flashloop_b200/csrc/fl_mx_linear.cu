@@ -177,7 +177,7 @@ struct Output {
 // Stores N rows of this thread's feature n, from row m on, of which `count` exist.  The 32 lanes of a
 // warp hold 32 consecutive features, which are one block of a microscaled result; whole warps call it.
 // WHOLE: all N rows exist.  That path has one branch at most: the epilogue of many rows is bound by the
-// instructions of its eight warps.
+// instructions of its warps.
 template <int KIND, bool WHOLE, int N>
 __device__ __forceinline__ void emit_rows(const Output& o, int64_t m, int n, const float (&v)[N], int count) {
   const bool live = n < o.features;
@@ -497,9 +497,15 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
 //
 // PACKED: both operands are e2m1.  They stay packed in shared memory, 256 elements to a stage, and go through
 // kind::mxf4, 64 elements an instruction at twice the rate (32768 x 5632 -> 2048: 139 us = 5440 TFLOP/s against 257 us
-// with x in mxfp8; gated 16384 x 2048 -> 5632: 210 against 270 us, where the epilogue is the longer part).
+// with x in mxfp8; gated 16384 x 2048 -> 5632: 164 against 266 us).
 
-constexpr int kPairThreads = 320;  // copies, matrix instructions, eight epilogue warps
+// Warps of the epilogue: with a gate to work out sixteen are faster than eight, without one slower (16384 x 2048 -> 5632
+// to mxfp8: 275 us with sixteen, 288 with eight, of 4-bit operands 177 and 235; 32768 x 2048 -> 6144: 325 us with sixteen, 292
+// with eight).
+template <bool DUAL>
+constexpr int kPairEpilogue = DUAL ? 16 : 8;
+template <bool DUAL>
+constexpr int kPairThreads = 64 + 32 * kPairEpilogue<DUAL>;  // and one each for copies and matrix instructions
 // NT: rows of x per tile.  A multiple of 64, as the scales of x start at an even column of tensor memory.
 constexpr int kPairRows = 192;
 constexpr int kPairXTiles = 2;  // scale tiles that 192 rows starting at a multiple of 64 touch
@@ -571,7 +577,7 @@ __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
 }
 
 template <int KIND, bool DUAL, bool PACKED>
-__global__ void __launch_bounds__(kPairThreads)
+__global__ void __launch_bounds__(kPairThreads<DUAL>)
 mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p) {
   using Shape = Pair<PACKED>;
   constexpr int kStages = Shape::kStages, kStageBytes = Shape::kStageBytes, kSteps = Shape::kSteps;
@@ -599,7 +605,7 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full + 8 * b, 1);
-      mbar_init(acc_empty + 8 * b, 16);  // a lane of each epilogue warp of both CTAs
+      mbar_init(acc_empty + 8 * b, 2 * kPairEpilogue<DUAL>);  // a lane of each epilogue warp of both CTAs
     }
     mbar_init(drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -703,15 +709,15 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
     __syncwarp();
     mbar_wait(drained, 0, p.steps);
   } else if (warp >= 2) {
-    const uint32_t quarter = uint32_t(warp & 3) * 32, half = uint32_t(warp - 2) / 4;
-    constexpr int kCols = kPairRows / 2;  // this warp's columns of a tile
-    const uint32_t mine = tmem + (quarter << 16) + half * kCols;
+    const uint32_t quarter = uint32_t(warp & 3) * 32, part = uint32_t(warp - 2) / 4;
+    constexpr int kCols = kPairRows / (kPairEpilogue<DUAL> / 4);  // this warp's columns of a tile
+    const uint32_t mine = tmem + (quarter << 16) + part * kCols;
     const uint32_t leader_empty = in_cta(acc_empty, 0);
     Ring acc_at;
     for (int64_t tile = pair; tile < p.units / kWeights; tile += pairs) {
       const int n0 = (int(tile % p.pair_tiles) * 2 + int(rank)) * 128;
       const int n = n0 + int(quarter) + lane;
-      const int64_t m0 = tile / p.pair_tiles * kPairRows + half * kCols;
+      const int64_t m0 = tile / p.pair_tiles * kPairRows + part * kCols;
       const int cols = n0 < p.out.features ? int(max(int64_t(0), min(int64_t(kCols), p.rows - m0))) : 0;
       const bool whole = cols == kCols;
       float gate[DUAL ? kCols : 1];
@@ -934,7 +940,7 @@ int launch_pairs(const LinearCall& call, int sms) {
   cudaError_t err = allow_shared_memory(kernel, allowed, call.device);
   // all of an SM's shared memory, as it takes all of its tensor memory (see above)
   if (err == cudaSuccess)
-    err = launch_overlapped(kernel, unsigned(2 * std::min<int64_t>(tiles, sms / 2)), kPairThreads, kSmemLimit, 2, call.stream,
+    err = launch_overlapped(kernel, unsigned(2 * std::min<int64_t>(tiles, sms / 2)), kPairThreads<DUAL>, kSmemLimit, 2, call.stream,
                             maps, p);
   if (err != cudaSuccess) {
     cudaGetLastError();
