@@ -24,10 +24,10 @@ MAX_COLUMNS = 2**31 - 256  # of a row: the kernels index a row in 32 bits
 
 
 def _format_code(name: str) -> int:
-    try:
-        return FORMATS[name]
-    except (KeyError, TypeError):
-        raise ValueError(f"unknown microscaled format {name!r}: use one of {sorted(FORMATS)}") from None
+    code = FORMATS.get(name) if isinstance(name, str) else None
+    if code is None:
+        raise ValueError(f"unknown microscaled format {name!r}: use one of {sorted(FORMATS)}")
+    return code
 
 
 def codes_shape(rows: int, cols: int, format: str) -> tuple[int, int]:
@@ -95,18 +95,20 @@ class MXTensor:
 
     @property
     def codes(self) -> torch.Tensor:
-        if self._codes is None:
-            rows, width = codes_shape(self.rows, self.cols, self.format)
-            self._codes = self._both.as_strided((rows, width), (width, 1))
-        return self._codes
+        codes = self._codes
+        if codes is None:
+            width = ((self.cols + 127) >> 7) * (64 if self._code else 128)
+            codes = self._codes = self._both.as_strided((self.rows, width), (width, 1))
+        return codes
 
     @property
     def scales(self) -> torch.Tensor:
-        if self._scales is None:
-            tiles, steps = (self.rows + 127) >> 7, (self.cols + 127) >> 7
-            self._scales = self._both.as_strided((tiles, steps, 32, 4, 4), (steps * 512, 512, 16, 4, 1),
-                                                 self.scales_ptr - self.codes_ptr)
-        return self._scales
+        scales = self._scales
+        if scales is None:
+            steps = (self.cols + 127) >> 7
+            scales = self._scales = self._both.as_strided(((self.rows + 127) >> 7, steps, 32, 4, 4),
+                                                          (steps * 512, 512, 16, 4, 1), self.scales_ptr - self.codes_ptr)
+        return scales
 
     def __reduce__(self):  # copies and pickles hold tensors of their own
         return MXTensor, (self.codes, self.scales, self.shape, self.format)

@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import copy
 import math
 import zlib
 
@@ -157,6 +158,29 @@ def test_norm(rows, width, dtype, fmt):
         bound = HALF_STEP[dtype] * want.abs() + 2.0 ** -24 * (width + 8) * (n.abs() + want.abs()) + 2.0 ** -25
         assert bool(((hidden.double() - want).abs() <= bound).all())
         _check_codes(q, _norm64(hidden.double(), w2, 1e-5), fmt)
+
+
+def test_norm_takes_strided_rows_and_leading_dimensions():
+    base = _random(12, 600, torch.bfloat16, "strided")
+    w = torch.ones(300, device="cuda", dtype=torch.bfloat16)
+    x, r = base[:, ::2], base[:1, 300:].expand(12, 300)
+    q, hidden, _ = fl.mx_rmsnorm(x, w, 1e-6, residual=r, weight2=w, eps2=1e-6)
+    same, other, _ = fl.mx_rmsnorm(x.contiguous().view(3, 4, 300), w, 1e-6, residual=r.contiguous().view(3, 4, 300), weight2=w,
+                                   eps2=1e-6)
+    assert same.shape == other.shape == (3, 4, 300) and torch.equal(other.view(12, 300), hidden)
+    assert torch.equal(q.codes, same.codes) and torch.equal(q.scales, same.scales)
+    one = fl.mx_rmsnorm(x[0], w, 1e-6)[0]
+    assert one.shape == (300,) and torch.equal(one.codes[0], fl.mx_rmsnorm(x, w, 1e-6)[0].codes[0])
+    empty, nothing, _ = fl.mx_rmsnorm(x[:0], w, 1e-6, weight2=w)
+    assert empty.shape == nothing.shape == (0, 300)
+
+
+def test_copies_hold_their_own_tensors():
+    q = fl.mx_quantize(_random(5, 200, torch.bfloat16, "copy"), "mxfp4")
+    twin = copy.deepcopy(q)
+    want = q.dequantize()
+    q.codes.zero_()
+    assert torch.equal(twin.dequantize(), want) and not q.dequantize().any()
 
 
 def test_norm_of_rows_that_are_zero_or_not_finite():
