@@ -476,10 +476,10 @@ extern "C" int fl_rmsnorm_mx(const void* x, const void* addend, const void* resi
   FL_REQUIRE(dtype_ok(dtype) && mx_format_ok(format), "%s: unknown type or format", who);
   FL_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && width > 0 && width <= kMaxNormWidth,
              "%s: width must be 1 to %d, got %d", who, kMaxNormWidth, width);
+  if (rows == 0) return FL_OK;  // an empty tensor has no address
   FL_REQUIRE((weight2 == nullptr) == (hidden == nullptr), "%s: weight2 and hidden go together", who);
   FL_REQUIRE(residual == nullptr || weight2 != nullptr, "%s: a residual needs weight2", who);
   FL_REQUIRE(sum_out == nullptr || addend != nullptr, "%s: sum_out needs an addend", who);
-  if (rows == 0) return FL_OK;
   FL_REQUIRE(x && weight && codes && scales, "%s: null argument", who);
   FL_REQUIRE(aligned16(codes) && aligned16(scales), "%s: codes and scales must be 16-byte aligned", who);
   return by_type_and_format(dtype, format,
