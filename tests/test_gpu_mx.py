@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import copy
 import math
+import threading
 import zlib
 
 import pytest
@@ -456,6 +457,28 @@ def test_long_rows():
         assert bool((y == cols).all())
         del x, w, y
     assert mx_status() == 0
+
+
+def test_calls_from_several_threads():
+    g = _gen("threads")
+    w = fl.mx_quantize(torch.randn(512, 512, generator=g, device="cuda"), "mxfp4")
+    inputs = [torch.randn(rows, 512, generator=g, device="cuda") for rows in (1, 16, 90, 9000)]
+    want = [fl.mx_linear(x, w) for x in inputs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                if not torch.equal(fl.mx_linear(inputs[i], w), want[i]):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and mx_status() == 0
 
 
 def test_gradients_are_refused():
