@@ -1,5 +1,6 @@
 // Quantisation to the microscaled formats, its inverse, and the RMSNorm that leaves its rows in one.
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 #include <type_traits>
 
@@ -12,16 +13,16 @@ constexpr int kMxThreads = 256;
 
 // Eight lanes take one step (128 elements) of a row, sixteen elements each: two lanes share a block, and
 // the four scale bytes of the step leave as one word.  A CTA takes UNROLL * 32 consecutive steps and asks for all of its elements before it uses any.
-template <typename T, int FORMAT, bool VEC, int UNROLL>
+template <typename T, int FORMAT, int ALIGN, int UNROLL>
 __global__ void __launch_bounds__(kMxThreads)
 quantize_kernel(const T* __restrict__ x, uint32_t rows, int cols, int64_t row_stride, uint32_t steps, uint32_t units,
                 uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   const uint32_t first = blockIdx.x * (UNROLL * kMxThreads / 8) + threadIdx.x / 8;
   const int lane = threadIdx.x & 7;
-  __shared__ __align__(16) WarpStage<T, VEC, kMxThreads> stage;
+  __shared__ __align__(16) WarpStage<T, ALIGN, kMxThreads> stage;
   wait_for_inputs();
   may_start_next();
-  Raw16<T> raw[UNROLL];
+  Load16<T, ALIGN> raw[UNROLL];
   uint32_t row[UNROLL];
   int e[UNROLL];
 #pragma unroll
@@ -29,14 +30,13 @@ quantize_kernel(const T* __restrict__ x, uint32_t rows, int cols, int64_t row_st
     const uint32_t unit = first + i * (kMxThreads / 8);
     row[i] = unit / steps;
     e[i] = int(unit - row[i] * steps) * kMxStep + lane * 16;
-    raw[i].template load<VEC>(x + int64_t(row[i]) * row_stride + e[i], unit < units && row[i] < rows ? cols - e[i] : 0,
-                               stage.mine());
+    raw[i].load(x + int64_t(row[i]) * row_stride + e[i], unit < units && row[i] < rows ? cols - e[i] : 0);
   }
 #pragma unroll
   for (int i = 0; i < UNROLL; ++i) {
     const uint32_t unit = first + i * (kMxThreads / 8);
     float v[16];
-    raw[i].unpack(v);
+    raw[i].get(stage.mine()).unpack(v);
     uint32_t out[4];
     const uint32_t word = mx_join_scales(mx_encode16<FORMAT>(v, out));
     if (unit >= units) continue;
@@ -50,13 +50,13 @@ quantize_kernel(const T* __restrict__ x, uint32_t rows, int cols, int64_t row_st
 }
 
 // Sixteen elements of a row per thread and round.
-template <typename T, int FORMAT, bool VEC, int UNROLL>
+template <typename T, int FORMAT, int ALIGN, int UNROLL>
 __global__ void __launch_bounds__(kMxThreads)
 dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int cols, uint32_t steps,
                   uint32_t units, T* __restrict__ out) {
   const uint32_t first = blockIdx.x * (UNROLL * kMxThreads / 8) + threadIdx.x / 8;
   const int lane = threadIdx.x & 7;
-  __shared__ __align__(16) WarpStage<T, VEC, kMxThreads> stage;
+  __shared__ __align__(16) WarpStage<T, ALIGN, kMxThreads> stage;
   wait_for_inputs();
   may_start_next();
   uint4 word[UNROLL] = {};
@@ -83,7 +83,7 @@ dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
   }
 #pragma unroll
   for (int i = 0; i < UNROLL; ++i) {
-    if (VEC && e[i] >= cols) continue;
+    if (ALIGN == 16 && e[i] >= cols) continue;
     const float scale = mx_scale_value(byte[i]);
     const uint32_t w[4] = {word[i].x, word[i].y, word[i].z, word[i].w};
     float v[16];
@@ -100,14 +100,12 @@ dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
       v[2 * k] = f.x * scale;
       v[2 * k + 1] = f.y * scale;
     }
-    store16<T, VEC>(out + int64_t(row[i]) * cols + e[i], cols - e[i], v, stage.mine());
+    store16<T, ALIGN>(out + int64_t(row[i]) * cols + e[i], cols - e[i], v, stage.mine());
   }
 }
 
-// Rows up to 8192 wide: eight warps of two chunks of sixteen elements per thread.
+// Rows up to 8192 wide: 256 threads of two chunks of sixteen elements.
 constexpr int kMaxNormWidth = 8192;
-constexpr int64_t kManyRows = 148 * 8;
-constexpr int kNormSmThreads = 768, kNormSmThreads2 = 512;  // threads of the persistent CTAs per SM, without and with weight2
 
 template <typename T>
 struct MxNormParams {
@@ -126,18 +124,19 @@ struct MxNormParams {
   uint8_t* scales;
 };
 
-// Sum over the warps of a row; every thread gets it.  `part` alternates between calls, so that one
-// barrier is enough.
-template <int WARPS>
+// Sum over the LANES threads of a row; every one of them gets it.
+template <int LANES>
 __device__ __forceinline__ float row_sum(float v, float* part) {
-  v = warp_sum(v);
-  if (WARPS == 1) return v;
-  const int warp = threadIdx.x >> 5, first = warp / WARPS * WARPS;
+#pragma unroll
+  for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (LANES <= 32) return v;
+  constexpr int kWarps = LANES / 32;
+  const int warp = threadIdx.x >> 5, first = warp / kWarps * kWarps;
   if ((threadIdx.x & 31) == 0) part[warp] = v;
   __syncthreads();
   float total = 0.f;
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) total += part[first + w];
+  for (int w = 0; w < kWarps; ++w) total += part[first + w];
   return total;
 }
 
@@ -162,93 +161,103 @@ __device__ __forceinline__ float inverse_root(float sum, int width, float eps) {
 // those of n; with it hidden = round([residual +] n) and the codes are those of weight2 * hidden *
 // rsqrt(mean(hidden^2) + eps2).  Everything between two stored tensors stays in float32.
 //
-// WARPS warps share a row and hold it in registers, CHUNKS times sixteen elements per thread.  Many
-// rows: CTAs of as few warps as hold a row, each taking row after row and asking for the next one before it works on
-// the present one; bound by memory (32768 x 2048 bfloat16 with residual and second norm: 80 us, 5.9 TB/s of the copy rate of
-// 6.5).  Few rows: a CTA each; bound by latency.
-template <int WARPS>
-constexpr int kNormThreads = WARPS < 4 ? 128 : WARPS * 32;
+// LANES threads share a row and hold it in registers, CHUNKS times sixteen elements per thread; as few as hold it, eight
+// (one scale word) at least.  CTAs take rows one after the other and ask for the next ones before they work on the
+// present ones: bound by memory with many rows (MEASURED), by latency with few.
+template <int LANES>
+constexpr int kNormThreads = LANES < 128 ? 128 : LANES;
 
-template <typename T, int CHUNKS, bool SECOND>
+template <typename T, int ALIGN, bool SECOND, int LANES, int CHUNKS>
 struct NormRow {
-  Raw16<T> x[CHUNKS], a[CHUNKS], r[SECOND ? CHUNKS : 1];
-  template <bool VEC, int ROW_THREADS>
-  __device__ __forceinline__ void load(const MxNormParams<T>& p, int64_t row, int thread, T* stage) {
+  Load16<T, ALIGN> x[CHUNKS], a[CHUNKS], r[SECOND ? CHUNKS : 1];
+  __device__ __forceinline__ void load(const MxNormParams<T>& p, int64_t row, int thread) {
     const int64_t base = row * p.width;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      const int e = (c * ROW_THREADS + thread) * 16, n = row < p.rows ? p.width - e : 0;
-      x[c].template load<VEC>(p.x + base + e, n, stage);
-      if (p.addend) a[c].template load<VEC>(p.addend + base + e, n, stage);
+      const int e = (c * LANES + thread) * 16, n = row < p.rows ? p.width - e : 0;
+      x[c].load(p.x + base + e, n);
+      if (p.addend) a[c].load(p.addend + base + e, n);
       if constexpr (SECOND) {
-        if (p.residual) r[c].template load<VEC>(p.residual + base + e, n, stage);
+        if (p.residual) r[c].load(p.residual + base + e, n);
       }
     }
   }
 };
 
 // SECOND: weight2 is given.
-template <typename T, int FORMAT, bool VEC, bool SECOND, int WARPS, int CHUNKS>
-__global__ void __launch_bounds__(kNormThreads<WARPS>) norm_mx_kernel(const MxNormParams<T> p) {
-  constexpr int kThreads = kNormThreads<WARPS>, kRowThreads = WARPS * 32, kRows = kThreads / kRowThreads;
+template <typename T, int FORMAT, int ALIGN, bool SECOND, int LANES, int CHUNKS>
+__global__ void __launch_bounds__(kNormThreads<LANES>) norm_mx_kernel(const MxNormParams<T> p) {
+  constexpr int kThreads = kNormThreads<LANES>, kRowThreads = LANES, kRows = kThreads / LANES;
   __shared__ float s_part[2][kThreads / 32];
-  __shared__ __align__(16) WarpStage<T, VEC, kThreads> stage;
+  __shared__ __align__(16) WarpStage<T, ALIGN, kThreads> stage;
   const int thread = threadIdx.x % kRowThreads;
   const int64_t stride = int64_t(gridDim.x) * kRows;
   const bool one_group = p.rows <= 32;  // a row's word is then the only one of its sixteen bytes
   int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / kRowThreads;
   wait_for_inputs();
   may_start_next();
-  NormRow<T, CHUNKS, SECOND> next;
-  next.template load<VEC, kRowThreads>(p, row, thread, stage.mine());
-  float w[CHUNKS][16], w2[SECOND ? CHUNKS : 1][16];
+  NormRow<T, ALIGN, SECOND, LANES, CHUNKS> next;
+  next.load(p, row, thread);
+  Raw16<T> raw_w[CHUNKS], raw_w2[SECOND ? CHUNKS : 1];
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
     const int e = (c * kRowThreads + thread) * 16;
-    load16<T, VEC>(p.weight + e, p.width - e, w[c], stage.mine());
-    if constexpr (SECOND) load16<T, VEC>(p.weight2 + e, p.width - e, w2[c], stage.mine());
+    Load16<T, ALIGN> w, w2;
+    w.load(p.weight + e, p.width - e);
+    if constexpr (SECOND) w2.load(p.weight2 + e, p.width - e);
+    raw_w[c] = w.get(stage.mine());
+    if constexpr (SECOND) raw_w2[c] = w2.get(stage.mine());
   }
   // the same number of rounds for all threads of the CTA, which meet at barriers
   for (int64_t first = int64_t(blockIdx.x) * kRows; first < p.rows; first += stride, row += stride) {
     const bool live = row < p.rows;
     const int64_t base = row * p.width;
-    NormRow<T, CHUNKS, SECOND> now = next;
-    if (first + stride < p.rows) next.template load<VEC, kRowThreads>(p, row + stride, thread, stage.mine());
+    Raw16<T> x[CHUNKS], a[CHUNKS], r[SECOND ? CHUNKS : 1];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      x[c] = next.x[c].get(stage.mine());
+      if (p.addend) a[c] = next.a[c].get(stage.mine());
+      if constexpr (SECOND) {
+        if (p.residual) r[c] = next.r[c].get(stage.mine());
+      }
+    }
+    if (first + stride < p.rows) next.load(p, row + stride, thread);
     float v[CHUNKS][16];
     float sq = 0.f;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      now.x[c].unpack(v[c]);
+      x[c].unpack(v[c]);
       if (p.addend) {
         const int e = (c * kRowThreads + thread) * 16, n = live ? p.width - e : 0;
-        float a[16];
-        now.a[c].unpack(a);
+        float add[16];
+        a[c].unpack(add);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[c][k] += a[k];
-        store16<T, VEC>(p.sum_out + base + e, p.sum_out ? n : 0, v[c], stage.mine());
+        for (int k = 0; k < 16; ++k) v[c][k] += add[k];
+        store16<T, ALIGN>(p.sum_out + base + e, p.sum_out ? n : 0, v[c], stage.mine());
       }
       sq += sum_of_squares(v[c]);
     }
-    float inv = inverse_root(row_sum<WARPS>(sq, s_part[0]), p.width, p.eps);
+    float inv = inverse_root(row_sum<LANES>(sq, s_part[0]), p.width, p.eps);
     sq = 0.f;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      float r[16] = {};
+      float res[16] = {}, w[16];
+      raw_w[c].unpack(w);
       if constexpr (SECOND) {
-        if (p.residual) now.r[c].unpack(r);
+        if (p.residual) r[c].unpack(res);
       }
 #pragma unroll
-      for (int k = 0; k < 16; ++k) v[c][k] = fmaf(w[c][k], v[c][k] * inv, r[k]);
+      for (int k = 0; k < 16; ++k) v[c][k] = fmaf(w[k], v[c][k] * inv, res[k]);
       if constexpr (SECOND) {
         const int e = (c * kRowThreads + thread) * 16, n = live ? p.width - e : 0;
-        store16<T, VEC>(p.hidden + base + e, n, v[c], stage.mine());
+        store16<T, ALIGN>(p.hidden + base + e, n, v[c], stage.mine());
         sq += sum_of_squares(v[c]);
       }
     }
     // one barrier per round orders the reads of s_part[0] before its next writes, and the second sum's does s_part[1]
     if constexpr (SECOND) {
-      inv = inverse_root(row_sum<WARPS>(sq, s_part[1]), p.width, p.eps2);
-    } else if (WARPS > 1) {
+      inv = inverse_root(row_sum<LANES>(sq, s_part[1]), p.width, p.eps2);
+    } else if (LANES > 32) {
       __syncthreads();
     }
     uint8_t* codes = p.codes + row * p.steps * (FORMAT == FL_MX_FP8 ? kMxStep : kMxStep / 2);
@@ -257,8 +266,10 @@ __global__ void __launch_bounds__(kNormThreads<WARPS>) norm_mx_kernel(const MxNo
       const int e = (c * kRowThreads + thread) * 16;
       const uint32_t step = uint32_t(e) / kMxStep;
       if constexpr (SECOND) {
+        float w[16];
+        raw_w2[c].unpack(w);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[c][k] = w2[c][k] * (v[c][k] * inv);
+        for (int k = 0; k < 16; ++k) v[c][k] = w[k] * (v[c][k] * inv);
       }
       if (e >= p.width) {  // padding is zero also where the row is not finite
 #pragma unroll
@@ -295,6 +306,16 @@ __global__ void __launch_bounds__(kNormThreads<WARPS>) norm_mx_kernel(const MxNo
 // Rounds per thread: several where that still leaves several CTAs to an SM, one below.
 constexpr int64_t kUnrollUnits = 148 * 8 * 64;
 
+// Calls f with the largest of 16, 4 and 2 bytes at whose multiples the addresses or-ed into `at` all lie.
+template <typename T, typename F>
+auto by_alignment(uintptr_t at, F&& f) {
+  if (at % 16 == 0) return f(std::integral_constant<int, 16>{});
+  if constexpr (sizeof(T) == 2) {
+    if (at % 4 != 0) return f(std::integral_constant<int, 2>{});
+  }
+  return f(std::integral_constant<int, 4>{});
+}
+
 int launched(cudaError_t err, const char* who) {
   if (err == cudaSuccess) return FL_OK;
   cudaGetLastError();
@@ -308,9 +329,12 @@ int launch_quantize(const void* x, int64_t rows, int32_t cols, int64_t stride, v
   const int64_t steps = mx_steps(cols);
   const int64_t units = (rows + kMxTileRows - 1) / kMxTileRows * kMxTileRows * steps;
   FL_REQUIRE(units < (int64_t(1) << 31), "fl_mx_quantize: too many elements");
-  const bool vec = aligned16(x) && (stride * sizeof(T) % 16 == 0 || rows == 1), many = units >= kUnrollUnits;
-  auto kernel = many ? (vec ? quantize_kernel<T, FORMAT, true, 2> : quantize_kernel<T, FORMAT, false, 2>)
-                     : (vec ? quantize_kernel<T, FORMAT, true, 1> : quantize_kernel<T, FORMAT, false, 1>);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(x) | (rows > 1 ? uintptr_t(stride) * sizeof(T) : 0);
+  const bool many = units >= kUnrollUnits;
+  auto kernel = by_alignment<T>(at % 16 == 0 ? 0 : at | uintptr_t(cols) * sizeof(T), [&](auto align) {
+    constexpr int kAlign = decltype(align)::value;
+    return many ? quantize_kernel<T, FORMAT, kAlign, 2> : quantize_kernel<T, FORMAT, kAlign, 1>;
+  });
   const int64_t each = (many ? 2 : 1) * (kMxThreads / 8);
   return launched(launch_overlapped(kernel, unsigned((units + each - 1) / each), kMxThreads, 0, 1, stream,
                                     static_cast<const T*>(x), uint32_t(rows), cols, stride, uint32_t(steps), uint32_t(units),
@@ -326,9 +350,11 @@ int launch_dequantize(const void* codes, const void* scales, int64_t rows, int32
   constexpr int kUnits = kMxThreads / 8;
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   const uint8_t* s = static_cast<const uint8_t*>(scales);
-  const bool many = units >= kUnrollUnits, vec = cols * sizeof(T) % 16 == 0;
-  auto kernel = many ? (vec ? dequantize_kernel<T, FORMAT, true, 4> : dequantize_kernel<T, FORMAT, false, 4>)
-                     : (vec ? dequantize_kernel<T, FORMAT, true, 1> : dequantize_kernel<T, FORMAT, false, 1>);
+  const bool many = units >= kUnrollUnits;
+  auto kernel = by_alignment<T>(uintptr_t(cols) * sizeof(T), [&](auto align) {
+    constexpr int kAlign = decltype(align)::value;
+    return many ? dequantize_kernel<T, FORMAT, kAlign, 4> : dequantize_kernel<T, FORMAT, kAlign, 1>;
+  });
   const int64_t each = many ? 4 * kUnits : kUnits;
   return launched(launch_overlapped(kernel, unsigned((units + each - 1) / each), kMxThreads, 0, 1, stream, c, s, cols,
                                     uint32_t(steps), uint32_t(units), static_cast<T*>(out)),
@@ -343,22 +369,29 @@ struct NormArgs {
   void *sum_out, *hidden, *codes, *scales;
 };
 
-template <typename T, int FORMAT, bool VEC, bool SECOND, int WARPS, int CHUNKS>
+template <typename T, int FORMAT, int ALIGN, bool SECOND, int LANES, int CHUNKS>
 cudaError_t launch_norm_shape(const MxNormParams<T>& p, cudaStream_t stream) {
-  constexpr int kThreads = kNormThreads<WARPS>, kRows = kThreads / 32 / WARPS;
-  const int64_t ctas = std::min<int64_t>((p.rows + kRows - 1) / kRows, 148 * ((SECOND ? kNormSmThreads2 : kNormSmThreads) / kThreads));
-  return launch_overlapped(norm_mx_kernel<T, FORMAT, VEC, SECOND, WARPS, CHUNKS>, unsigned(ctas), kThreads, 0, 1, stream, p);
+  constexpr int kThreads = kNormThreads<LANES>, kRows = kThreads / LANES;
+  auto kernel = norm_mx_kernel<T, FORMAT, ALIGN, SECOND, LANES, CHUNKS>;
+  static std::atomic<int> fit;  // CTAs that run on an SM at once, asked once
+  int ctas = fit.load(std::memory_order_relaxed);
+  if (ctas == 0) {
+    const cudaError_t err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, kThreads, 0);
+    if (err != cudaSuccess) return err;
+    fit.store(ctas, std::memory_order_relaxed);
+  }
+  return launch_overlapped(kernel, unsigned(std::min<int64_t>((p.rows + kRows - 1) / kRows, 148 * ctas)), kThreads, 0, 1, stream, p);
 }
 
-// Warps to a row: as few as hold it once there are rows enough to fill the SMs, otherwise eight.
-template <typename T, int FORMAT, bool VEC, bool SECOND>
+template <typename T, int FORMAT, int ALIGN, bool SECOND>
 cudaError_t launch_norm_rows(const MxNormParams<T>& p, cudaStream_t stream) {
-  const bool many = p.rows >= kManyRows;
-  if (many && p.width <= 512) return launch_norm_shape<T, FORMAT, VEC, SECOND, 1, 1>(p, stream);
-  if (many && p.width <= 1024) return launch_norm_shape<T, FORMAT, VEC, SECOND, 2, 1>(p, stream);
-  if (p.width <= 2048) return launch_norm_shape<T, FORMAT, VEC, SECOND, 4, 1>(p, stream);
-  if (p.width <= 4096) return launch_norm_shape<T, FORMAT, VEC, SECOND, 8, 1>(p, stream);
-  return launch_norm_shape<T, FORMAT, VEC, SECOND, 8, 2>(p, stream);
+  if (p.width <= 128) return launch_norm_shape<T, FORMAT, ALIGN, SECOND, 8, 1>(p, stream);
+  if (p.width <= 256) return launch_norm_shape<T, FORMAT, ALIGN, SECOND, 16, 1>(p, stream);
+  if (p.width <= 512) return launch_norm_shape<T, FORMAT, ALIGN, SECOND, 32, 1>(p, stream);
+  if (p.width <= 1024) return launch_norm_shape<T, FORMAT, ALIGN, SECOND, 64, 1>(p, stream);
+  if (p.width <= 2048) return launch_norm_shape<T, FORMAT, ALIGN, SECOND, 128, 1>(p, stream);
+  if (p.width <= 4096) return launch_norm_shape<T, FORMAT, ALIGN, SECOND, 256, 1>(p, stream);
+  return launch_norm_shape<T, FORMAT, ALIGN, SECOND, 256, 2>(p, stream);
 }
 
 template <typename T, int FORMAT>
@@ -378,15 +411,14 @@ int launch_norm(const NormArgs& a, cudaStream_t stream) {
   p.hidden = static_cast<T*>(a.hidden);
   p.codes = static_cast<uint8_t*>(a.codes);
   p.scales = static_cast<uint8_t*>(a.scales);
-  const bool vec = aligned16(a.x) && aligned16(a.addend) && aligned16(a.residual) && aligned16(a.weight) &&
-                   aligned16(a.weight2) && aligned16(a.sum_out) && aligned16(a.hidden) &&
-                   a.width * sizeof(T) % 16 == 0;
-  cudaError_t err;
-  if (vec) {
-    err = a.weight2 ? launch_norm_rows<T, FORMAT, true, true>(p, stream) : launch_norm_rows<T, FORMAT, true, false>(p, stream);
-  } else {
-    err = a.weight2 ? launch_norm_rows<T, FORMAT, false, true>(p, stream) : launch_norm_rows<T, FORMAT, false, false>(p, stream);
-  }
+  uintptr_t at = uintptr_t(a.width) * sizeof(T);
+  for (const void* q : {a.x, a.addend, a.residual, a.weight, a.weight2, static_cast<const void*>(a.sum_out),
+                        static_cast<const void*>(a.hidden)})
+    at |= reinterpret_cast<uintptr_t>(q);
+  const cudaError_t err = by_alignment<T>(at, [&](auto align) {
+    constexpr int kAlign = decltype(align)::value;
+    return a.weight2 ? launch_norm_rows<T, FORMAT, kAlign, true>(p, stream) : launch_norm_rows<T, FORMAT, kAlign, false>(p, stream);
+  });
   return launched(err, "fl_rmsnorm_mx");
 }
 

@@ -139,61 +139,11 @@ __device__ __forceinline__ uint32_t mx_join_scales(uint32_t byte) {
   return word | __shfl_xor_sync(0xffffffffu, word, 4);
 }
 
-// Sixteen consecutive elements as they lie in memory, so that a load can be under way while others are
-// used.  `count` of them exist (none if it is not positive), the others are zero.
-// VEC: loads of 16 bytes (the caller has checked the alignment of the base and of the row stride), of 32
-// where the address allows.  Otherwise the warp, whose groups of eight lanes each hold 128 consecutive
-// elements, loads them lane by lane and passes them on through 512 elements of shared memory, `stage`; all of its
-// lanes make the call.
+// Sixteen consecutive elements as they lie in memory.
 template <typename T>
 struct Raw16 {
   static constexpr int kWords = 4 * sizeof(T);  // of four bytes
   uint32_t w[kWords];
-  template <bool VEC>
-  __device__ __forceinline__ void load(const T* p, int count, T* stage) {
-    if constexpr (VEC) {
-      if (count >= 16) {
-        if ((reinterpret_cast<uintptr_t>(p) & 31) == 0) {
-#pragma unroll
-          for (int i = 0; i < kWords; i += 8)
-            asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]),
-                  "=r"(w[i + 6]), "=r"(w[i + 7])
-                : "l"(reinterpret_cast<const uint32_t*>(p) + i));
-        } else {
-#pragma unroll
-          for (int i = 0; i < kWords; i += 4) {
-            const uint4 q = ldg128(reinterpret_cast<const uint32_t*>(p) + i);
-            w[i] = q.x, w[i + 1] = q.y, w[i + 2] = q.z, w[i + 3] = q.w;
-          }
-        }
-      } else {
-        T t[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) t[k] = k < count ? p[k] : T(0.f);
-        memcpy(w, t, sizeof(t));
-      }
-    } else {
-      const int lane = threadIdx.x & 31;
-      T t[16];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const T* base = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(p), g * 8));
-        const int total = __shfl_sync(0xffffffffu, count, g * 8);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t[4 * g + i] = lane + 32 * i < total ? base[lane + 32 * i] : T(0.f);
-      }
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 16; ++i) stage[lane + 32 * i] = t[i];
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < kWords; i += 4) {
-        const uint4 q = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(stage) + lane * kWords + i);
-        w[i] = q.x, w[i + 1] = q.y, w[i + 2] = q.z, w[i + 3] = q.w;
-      }
-    }
-  }
   __device__ __forceinline__ void unpack(float (&v)[16]) const {
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
@@ -207,13 +157,78 @@ struct Raw16 {
     }
   }
 };
-template <typename T, bool VEC>
-__device__ __forceinline__ void load16(const T* p, int count, float (&v)[16], T* stage) {
-  Raw16<T> raw;
-  raw.template load<VEC>(p, count, stage);
-  raw.unpack(v);
-}
 
+// A load of Raw16 that can be under way while others are used: load() asks, get() waits.  `count` of the elements
+// exist (none if it is not positive), the others are zero.
+// ALIGN: the bytes at whose multiples base and row stride are known to lie.  16: loads of 16 bytes, of 32
+// where the address allows.  Less: the warp, whose groups of eight lanes each hold 128 consecutive elements, loads
+// them ALIGN bytes (and the rows' lengths are multiples of that) lane by lane and passes them on through 512 elements of
+// shared memory, `stage`; all of its lanes make both calls.
+template <typename T, int ALIGN>
+struct Load16 {
+  using Piece = std::conditional_t<ALIGN == 2, uint16_t, uint32_t>;
+  static constexpr int kOfPiece = ALIGN / sizeof(T);    // elements
+  static constexpr int kPieces = 128 / 32 / kOfPiece;   // of a lane and group
+  uint32_t t[4 * kPieces];
+  __device__ __forceinline__ void load(const T* p, int count) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const Piece* q = reinterpret_cast<const Piece*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(p), g * 8));
+      const int total = __shfl_sync(0xffffffffu, count, g * 8);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        t[g * kPieces + i] = (lane + 32 * i) * kOfPiece < total ? __ldg(q + lane + 32 * i) : 0u;
+    }
+  }
+  __device__ __forceinline__ Raw16<T> get(T* stage) const {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4 * kPieces; ++i) reinterpret_cast<Piece*>(stage)[lane + 32 * i] = Piece(t[i]);
+    __syncwarp();
+    Raw16<T> raw;
+#pragma unroll
+    for (int i = 0; i < Raw16<T>::kWords; i += 4) {
+      const uint4 q = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(stage) + lane * Raw16<T>::kWords + i);
+      raw.w[i] = q.x, raw.w[i + 1] = q.y, raw.w[i + 2] = q.z, raw.w[i + 3] = q.w;
+    }
+    return raw;
+  }
+};
+template <typename T>
+struct Load16<T, 16> {
+  Raw16<T> raw;
+  __device__ __forceinline__ void load(const T* p, int count) {
+    constexpr int kWords = Raw16<T>::kWords;
+    uint32_t (&w)[kWords] = raw.w;
+    if (count >= 16 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 8)
+        asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+            : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]),
+              "=r"(w[i + 6]), "=r"(w[i + 7])
+            : "l"(reinterpret_cast<const uint32_t*>(p) + i));
+      return;
+    }
+    constexpr int kEach = 16 / sizeof(T);  // elements of 16 bytes
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4) {
+      const int at = i / 4 * kEach, left = count - at;
+      uint4 q = make_uint4(0u, 0u, 0u, 0u);
+      if (left >= kEach) {
+        q = ldg128(p + at);
+      } else if (left > 0) {  // rows that end inside 16 bytes
+        T t[kEach];
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) t[k] = k < left ? p[at + k] : T(0.f);
+        memcpy(&q, t, sizeof(t));
+      }
+      w[i] = q.x, w[i + 1] = q.y, w[i + 2] = q.z, w[i + 3] = q.w;
+    }
+  }
+  __device__ __forceinline__ Raw16<T> get(T*) const { return raw; }
+};
 template <typename T>
 __device__ __forceinline__ T round_to(float v);
 template <>
@@ -242,13 +257,13 @@ __device__ __forceinline__ Raw16<T> pack16(const float (&v)[16]) {
 }
 
 // The first `count` of sixteen values (none if it is not positive) rounded to T and stored; `v` becomes what
-// they are rounded to.  VEC, `stage` and the call by whole warps as for the load.
-template <typename T, bool VEC>
+// they are rounded to.  ALIGN, `stage` and the call by whole warps as for the load.
+template <typename T, int ALIGN>
 __device__ __forceinline__ void store16(T* p, int count, float (&v)[16], T* stage) {
   const Raw16<T> raw = pack16<T>(v);
   raw.unpack(v);
   const uint32_t* w = raw.w;
-  if constexpr (VEC) {
+  if constexpr (ALIGN == 16) {
     uint32_t* q = reinterpret_cast<uint32_t*>(p);
     if (count >= 16 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
 #pragma unroll
@@ -256,16 +271,21 @@ __device__ __forceinline__ void store16(T* p, int count, float (&v)[16], T* stag
         asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
                      ::"l"(q + i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]),
                        "r"(w[i + 6]), "r"(w[i + 7]) : "memory");
-    } else if (count >= 16) {
-#pragma unroll
-      for (int i = 0; i < Raw16<T>::kWords; i += 4)
-        *reinterpret_cast<uint4*>(q + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
     } else {
-      T t[16];
-      memcpy(t, w, sizeof(t));
+      constexpr int kEach = 16 / sizeof(T);
 #pragma unroll
-      for (int k = 0; k < 16; ++k)
-        if (k < count) p[k] = t[k];
+      for (int i = 0; i < Raw16<T>::kWords; i += 4) {
+        const int at = i / 4 * kEach, left = count - at;
+        if (left >= kEach) {
+          *reinterpret_cast<uint4*>(q + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        } else if (left > 0) {
+          T t[kEach];
+          memcpy(t, w + i, sizeof(t));
+#pragma unroll
+          for (int k = 0; k < kEach; ++k)
+            if (k < left) p[at + k] = t[k];
+        }
+      }
     }
   } else {
     const int lane = threadIdx.x & 31;
@@ -275,20 +295,23 @@ __device__ __forceinline__ void store16(T* p, int count, float (&v)[16], T* stag
       *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(stage) + lane * Raw16<T>::kWords + i) =
           make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
     __syncwarp();
+    using Piece = typename Load16<T, ALIGN>::Piece;
+    constexpr int kOfPiece = Load16<T, ALIGN>::kOfPiece, kPieces = Load16<T, ALIGN>::kPieces;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      T* base = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(p), g * 8));
+      Piece* base = reinterpret_cast<Piece*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(p), g * 8));
       const int total = __shfl_sync(0xffffffffu, count, g * 8);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (lane + 32 * i < total) base[lane + 32 * i] = stage[g * 128 + lane + 32 * i];
+      for (int i = 0; i < kPieces; ++i)
+        if ((lane + 32 * i) * kOfPiece < total)
+          base[lane + 32 * i] = reinterpret_cast<const Piece*>(stage)[(g * kPieces + i) * 32 + lane];
     }
   }
 }
-// Shared memory of the warps for loads and stores without VEC.
-template <typename T, bool VEC, int THREADS>
+// Shared memory of the warps for loads and stores of less than 16 bytes.
+template <typename T, int ALIGN, int THREADS>
 struct WarpStage {
-  T data[THREADS / 32][VEC ? 16 : 512];
+  T data[THREADS / 32][ALIGN == 16 ? 16 : 512];
   __device__ __forceinline__ T* mine() { return data[threadIdx.x >> 5]; }
 };
 
