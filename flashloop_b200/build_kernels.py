@@ -17,9 +17,11 @@ from pathlib import Path
 CSRC = Path(__file__).resolve().parent / "csrc"
 LIBRARY = CSRC / "libflashloop_b200.so"
 SOURCES = ("fl_capi.cu", "fl_pack.cu", "fl_reader.cu", "fl_selected.cu", "fl_select.cu", "fl_append.cu", "fl_compact.cu",
-           "fl_step.cu", "fl_encode.cu", "fl_comm.cu", "fl_linear.cu", "fl_mx.cu", "fl_mx_linear.cu")
+           "fl_step.cu", "fl_encode.cu", "fl_comm.cu", "fl_linear.cu", "fl_mx.cu", "fl_mx_norm.cu", "fl_mx_linear.cu")
 FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
          "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr")
+# many small kernels in one file: its back end runs on several threads
+EXTRA_FLAGS = {"fl_mx_norm.cu": ("--split-compile", "0")}
 
 
 def _nvcc() -> str:
@@ -48,7 +50,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         obj = src.with_suffix(".o")
         objects.append(obj)
         if force or _stale(obj, [src, *headers]):
-            cmd = [nvcc, *FLAGS, "-c", str(src), "-o", str(obj)]
+            cmd = [nvcc, *FLAGS, *EXTRA_FLAGS.get(src.name, ()), "-c", str(src), "-o", str(obj)]
             if verbose:
                 cmd.insert(1, "-Xptxas")
                 cmd.insert(2, "-v")

@@ -1,4 +1,4 @@
-// Microscaled formats shared by the quantiser and norm (fl_mx.cu) and the projections
+// Microscaled formats shared by the quantiser (fl_mx.cu), the norm (fl_mx_norm.cu) and the projections
 // (fl_mx_linear.cu): blocks of 32 elements along a row, each with a power-of-two scale (e8m0: byte b
 // stands for 2^(b - 127), 255 for NaN) and elements of eight bits (e4m3) or four (e2m1).
 //
@@ -324,6 +324,40 @@ __device__ __forceinline__ void store_codes(uint8_t* row_codes, int64_t e, const
     *reinterpret_cast<uint2*>(row_codes + e / 2) = make_uint2(codes[0], codes[1]);
   }
 }
+
+// ------------------------------------------------------------------------------ host side
+
+// Calls f with the largest of 16, 4 and 2 bytes at whose multiples the addresses or-ed into `at` all lie.
+template <typename T, typename F>
+auto by_alignment(uintptr_t at, F&& f) {
+  if (at % 16 == 0) return f(std::integral_constant<int, 16>{});
+  if constexpr (sizeof(T) == 2) {
+    if (at % 4 != 0) return f(std::integral_constant<int, 2>{});
+  }
+  return f(std::integral_constant<int, 4>{});
+}
+
+inline int launched(cudaError_t err, const char* who) {
+  if (err == cudaSuccess) return FL_OK;
+  cudaGetLastError();
+  set_error("%s: %s", who, cudaGetErrorString(err));
+  return FL_ERR_CUDA;
+}
+
+// Calls f.template run<T, FORMAT>() for the type and format codes (validated by the caller).
+template <typename F>
+int by_type_and_format(int dtype, int format, F&& f) {
+  const bool fp8 = format == FL_MX_FP8;
+  switch (dtype) {
+    case FL_DTYPE_BF16:
+      return fp8 ? f.template run<__nv_bfloat16, FL_MX_FP8>() : f.template run<__nv_bfloat16, FL_MX_FP4>();
+    case FL_DTYPE_F16:
+      return fp8 ? f.template run<__half, FL_MX_FP8>() : f.template run<__half, FL_MX_FP4>();
+    default:
+      return fp8 ? f.template run<float, FL_MX_FP8>() : f.template run<float, FL_MX_FP4>();
+  }
+}
+inline bool dtype_ok(int dtype) { return dtype == FL_DTYPE_BF16 || dtype == FL_DTYPE_F16 || dtype == FL_DTYPE_F32; }
 
 #endif  // __CUDACC__
 
