@@ -1,5 +1,5 @@
 """Microscaled operands: quantisation, the norm that writes them, and the projections that take them
-(``csrc/fl_mx.cu``, ``csrc/fl_mx_linear.cu``).
+(``csrc/fl_mx.cu``, ``csrc/fl_mx_norm.cu``, ``csrc/fl_mx_linear.cu``).
 
 Thirty-two consecutive elements of a row share a power-of-two scale; the elements are e4m3
 (``"mxfp8"``) or e2m1 (``"mxfp4"``).  The reference's projections are bfloat16
