@@ -88,6 +88,38 @@ class MXTensor:
         self.scales_ptr = self.codes_ptr + at
         return self
 
+    @classmethod
+    def from_row_scales(cls, codes: torch.Tensor, scales: torch.Tensor, shape, format: str) -> "MXTensor":
+        """From the plain layout of a checkpoint: ``codes`` [rows, cols] (mxfp8) or [rows, ceil(cols / 2)] (mxfp4, the
+        even element in the low nibble) and ``scales`` [rows, ceil(cols / 32)], uint8 or the float8 types of the
+        same bytes; padded and tiled once, by tensor operations on whatever device they are."""
+
+        shape = tuple(int(v) for v in shape)
+        if not shape or min(shape) < 0 or not 0 < shape[-1] <= MAX_COLUMNS:
+            raise ValueError(f"a microscaled tensor needs a last dimension of 1 to {MAX_COLUMNS}")
+        rows, cols, code = math.prod(shape[:-1]), shape[-1], _format_code(format)
+        for t, want, name in ((codes, (rows, -(-cols // 2) if code else cols), "codes"),
+                              (scales, (rows, -(-cols // 32)), "scales")):
+            if t.element_size() != 1 or tuple(t.shape) != want:
+                raise ValueError(f"{name} of {shape} in {format} must be one byte each, {want}, got {tuple(t.shape)} {t.dtype}")
+        codes, scales = codes.view(torch.uint8), scales.view(torch.uint8)
+        if code and cols % 2:
+            codes = codes.clone()
+            codes[:, -1] &= 15  # the element past the last column
+        tiles, steps = -(-rows // 128), -(-cols // 128)
+        pad = torch.nn.functional.pad
+        codes = pad(codes, (0, codes_shape(rows, cols, format)[1] - codes.shape[1])).contiguous()
+        scales = pad(scales, (0, steps * 4 - scales.shape[1], 0, tiles * 128 - rows))
+        scales = scales.view(tiles, 4, 32, steps, 4).permute(0, 3, 2, 1, 4).contiguous()
+        return cls(codes, scales, shape, format)
+
+    def row_scales(self) -> torch.Tensor:
+        """The scale bytes as [rows, ceil(cols / 32)]."""
+
+        tiles, steps = scales_shape(self.rows, self.cols)[:2]
+        plain = self.scales.permute(0, 3, 2, 1, 4).reshape(tiles * 128, steps * 4)
+        return plain[:self.rows, :-(-self.cols // 32)].contiguous()
+
     def _any(self) -> torch.Tensor:
         """A tensor of this one's device, to allocate beside."""
 

@@ -58,6 +58,28 @@ def test_container_checks():
         fl.MXTensor(codes, scales, (), "mxfp8")
 
 
+@pytest.mark.parametrize("rows,cols,fmt", [(1, 1, "mxfp4"), (5, 33, "mxfp4"), (130, 200, "mxfp8"), (300, 257, "mxfp4"), (0, 64, "mxfp8")])
+def test_plain_layout_of_a_checkpoint(rows, cols, fmt):
+    g = torch.Generator().manual_seed(rows + cols)
+    width = -(-cols // 2) if fmt == "mxfp4" else cols
+    codes = torch.randint(0, 120, (rows, width), generator=g, dtype=torch.uint8)  # no NaN of e4m3
+    scales = torch.randint(100, 150, (rows, -(-cols // 32)), generator=g, dtype=torch.uint8)
+    t = fl.MXTensor.from_row_scales(codes, scales, (rows, cols), fmt)
+    assert torch.equal(t.row_scales(), scales)
+    values = codes.long()
+    if fmt == "mxfp4":
+        values = torch.stack((values & 15, values >> 4), -1).view(rows, -1)[:, :cols]
+    half = 8 if fmt == "mxfp4" else 128
+    grid = ref.grid(fmt)
+    want = torch.where(values >= half, -1.0, 1.0) * grid[values % half]
+    want = want * (2.0 ** (scales.double() - 127)).repeat_interleave(32, 1)[:, :cols]
+    assert torch.equal(ref.decode(t.codes, t.scales, fmt, rows, cols), want)
+    assert not ref.decode(t.codes, t.scales, fmt, rows, t.codes.shape[1] * (2 if fmt == "mxfp4" else 1))[:, cols:].any()
+    assert not ref.scale_bytes(t.scales, rows)[rows:].any()
+    with pytest.raises(ValueError, match="scales"):
+        fl.MXTensor.from_row_scales(codes, scales[:, :-1], (rows, cols), fmt)
+
+
 def test_rows_that_no_index_reaches_are_refused():
     wide = torch.zeros(1, dtype=torch.bfloat16).expand(2**32 + 64)  # one element of memory
     with pytest.raises(ValueError, match="columns"):
