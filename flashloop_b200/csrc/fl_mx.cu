@@ -15,8 +15,8 @@ constexpr int kMxThreads = 256;
 // 5631, which go through shared memory, 60 us.
 template <typename T, int FORMAT, int ALIGN, int UNROLL>
 __global__ void __launch_bounds__(kMxThreads)
-quantize_kernel(const T* __restrict__ x, uint32_t rows, int cols, int64_t row_stride, uint32_t steps, uint32_t units,
-                uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+quantize_kernel(const T* x, uint32_t rows, int cols, int64_t row_stride, uint32_t steps, uint32_t units,
+                uint8_t* codes, uint8_t* scales) {
   const uint32_t first = blockIdx.x * (UNROLL * kMxThreads / 8) + threadIdx.x / 8;
   const int lane = threadIdx.x & 7;
   __shared__ __align__(16) WarpStage<T, ALIGN, kMxThreads> stage;
@@ -52,8 +52,8 @@ quantize_kernel(const T* __restrict__ x, uint32_t rows, int cols, int64_t row_st
 // Sixteen elements of a row per thread and round.
 template <typename T, int FORMAT, int ALIGN, int UNROLL>
 __global__ void __launch_bounds__(kMxThreads)
-dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int cols, uint32_t steps,
-                  uint32_t units, T* __restrict__ out) {
+dequantize_kernel(const uint8_t* codes, const uint8_t* scales, int cols, uint32_t steps,
+                  uint32_t units, T* out) {
   const uint32_t first = blockIdx.x * (UNROLL * kMxThreads / 8) + threadIdx.x / 8;
   const int lane = threadIdx.x & 7;
   __shared__ __align__(16) WarpStage<T, ALIGN, kMxThreads> stage;
@@ -72,13 +72,13 @@ dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
     if (e[i] < cols) {
       const uint8_t* src = codes + int64_t(unit) * (FORMAT == FL_MX_FP8 ? kMxStep : kMxStep / 2);
       if (FORMAT == FL_MX_FP8) {
-        word[i] = ldg128(src + lane * 16);
+        word[i] = load_uint4(src + lane * 16);
       } else {
-        const uint2 half = ldg64(src + lane * 8);
+        const uint2 half = load_uint2(src + lane * 8);
         word[i].x = half.x;
         word[i].y = half.y;
       }
-      byte[i] = __ldg(scales + mx_scale_offset(row[i], step, steps) + lane / 2);
+      byte[i] = load_piece(scales + mx_scale_offset(row[i], step, steps) + lane / 2);
     }
   }
 #pragma unroll

@@ -40,6 +40,40 @@ inline bool mx_format_ok(int format) { return format == FL_MX_FP8 || format == F
 __device__ __forceinline__ void wait_for_inputs() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void may_start_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Loads of the caller's data in these kernels.  The kernel before may still be writing it when this one
+// starts, so it is not constant for the kernel's life (no ld.global.nc, no __ldg), and nothing may
+// move such a load in front of wait_for_inputs(): volatile, with a memory clobber as the wait has.
+__device__ __forceinline__ void load_words(const void* p, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d, uint32_t& e,
+                                           uint32_t& f, uint32_t& g, uint32_t& h) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(a), "=r"(b), "=r"(c), "=r"(d), "=r"(e), "=r"(f), "=r"(g), "=r"(h) : "l"(p) : "memory");
+}
+__device__ __forceinline__ uint4 load_uint4(const void* p) {
+  uint4 q;
+  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "l"(p) : "memory");
+  return q;
+}
+__device__ __forceinline__ uint2 load_uint2(const void* p) {
+  uint2 q;
+  asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(q.x), "=r"(q.y) : "l"(p) : "memory");
+  return q;
+}
+__device__ __forceinline__ uint32_t load_piece(const uint32_t* p) {
+  uint32_t v;
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t load_piece(const uint16_t* p) {
+  uint16_t v;
+  asm volatile("ld.global.b16 %0, [%1];" : "=h"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t load_piece(const uint8_t* p) {
+  uint32_t v;
+  asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
 template <typename... Params, typename... Args>
 cudaError_t launch_overlapped(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem, unsigned cluster,
                               cudaStream_t stream, Args&&... args) {
@@ -178,7 +212,7 @@ struct Load16 {
       const int total = __shfl_sync(0xffffffffu, count, g * 8);
 #pragma unroll
       for (int i = 0; i < kPieces; ++i)
-        t[g * kPieces + i] = (lane + 32 * i) * kOfPiece < total ? __ldg(q + lane + 32 * i) : 0u;
+        t[g * kPieces + i] = (lane + 32 * i) * kOfPiece < total ? load_piece(q + lane + 32 * i) : 0u;
     }
   }
   __device__ __forceinline__ Raw16<T> get(T* stage) const {
@@ -205,10 +239,8 @@ struct Load16<T, 16> {
     if (count >= 16 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
 #pragma unroll
       for (int i = 0; i < kWords; i += 8)
-        asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-            : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]),
-              "=r"(w[i + 6]), "=r"(w[i + 7])
-            : "l"(reinterpret_cast<const uint32_t*>(p) + i));
+        load_words(reinterpret_cast<const uint32_t*>(p) + i, w[i], w[i + 1], w[i + 2], w[i + 3], w[i + 4], w[i + 5],
+                   w[i + 6], w[i + 7]);
       return;
     }
     constexpr int kEach = 16 / sizeof(T);  // elements of 16 bytes
@@ -217,11 +249,13 @@ struct Load16<T, 16> {
       const int at = i / 4 * kEach, left = count - at;
       uint4 q = make_uint4(0u, 0u, 0u, 0u);
       if (left >= kEach) {
-        q = ldg128(p + at);
+        q = load_uint4(p + at);
       } else if (left > 0) {  // rows that end inside 16 bytes
-        T t[kEach];
+        using Bits = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>;
+        Bits t[kEach];
 #pragma unroll
-        for (int k = 0; k < kEach; ++k) t[k] = k < left ? p[at + k] : T(0.f);
+        for (int k = 0; k < kEach; ++k)
+          t[k] = k < left ? Bits(load_piece(reinterpret_cast<const Bits*>(p) + at + k)) : Bits(0);
         memcpy(&q, t, sizeof(t));
       }
       w[i] = q.x, w[i + 1] = q.y, w[i + 2] = q.z, w[i + 3] = q.w;
