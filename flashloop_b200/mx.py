@@ -47,7 +47,7 @@ class MXTensor:
     """A tensor whose last dimension is held in a microscaled format.
 
     ``codes`` uint8 (:func:`codes_shape`, elements past the last column zero) and ``scales`` uint8
-    (:func:`scales_shape`, rows past the last zero; byte b stands for 2^(b - 127), 255 for NaN) of
+    (:func:`scales_shape`, rows and blocks past the last zero; byte b stands for 2^(b - 127), 255 for NaN) of
     ``shape``, whose leading dimensions are the rows.  The tensors are held, not copied."""
 
     __slots__ = ("shape", "format", "rows", "cols", "device", "codes_ptr", "scales_ptr", "_code", "_codes", "_scales",
