@@ -53,12 +53,13 @@ __device__ __forceinline__ float sum_of_squares(const float (&v)[16]) {
 }
 
 // 1 / sqrt(mean + eps): the hardware's root and one Newton step, so that the float32 result carries the rounding
-// of its products only.
+// of its products only.  The step is for a finite, positive mean: of an infinite one (an infinity in the row, or
+// squares past float32's range) the factor is 0, of zero it is infinite, of a NaN a NaN.
 __device__ __forceinline__ float inverse_root(float sum, int width, float eps) {
   const float m = sum / float(width) + eps;
   const float y = rsqrtf(m);
   const float r = fmaf(-m * y, y, 1.f);
-  return isfinite(y) ? fmaf(0.5f * y, r, y) : y;
+  return y > 0.f && isfinite(y) ? fmaf(0.5f * y, r, y) : y;
 }
 
 // s = round(addend + x) or x;  n = weight * s * rsqrt(mean(s^2) + eps).  Without weight2 the codes are
