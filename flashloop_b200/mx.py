@@ -152,8 +152,10 @@ class MXTensor:
         return self.codes.numel() + self.scales.numel()
 
     def view(self, *shape) -> "MXTensor":
-        """The same rows under other leading dimensions."""
+        """The same rows under other leading dimensions; the last one stays (what lies past it is zero)."""
 
+        if not shape or int(shape[-1]) != self.cols:
+            raise ValueError(f"a view keeps the last dimension, {self.cols}, got {shape}")
         return MXTensor(self.codes, self.scales, shape, self.format)
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
