@@ -1036,6 +1036,14 @@ template <bool DUAL>
 int run_linear(LinearCall call) {
   FL_REQUIRE(cudaGetDevice(&call.device) == cudaSuccess && call.device >= 0 && call.device < kMaxDevices,
              "%s: no current device", call.who);
+  // Tensor maps are encoded by the driver, which wants the device's context current in this thread: the runtime
+  // binds it at a thread's first launch, and this call may be the first thing that a thread does.  Once per thread
+  // and change of device, as it takes 0.3 us.
+  thread_local int bound = -1;
+  if (bound != call.device) {
+    FL_REQUIRE(cudaSetDevice(call.device) == cudaSuccess, "%s: device %d has no context", call.who, call.device);
+    bound = call.device;
+  }
   switch (call.out_kind) {
     case kOutBf16: return choose_linear<kOutBf16, DUAL>(call);
     case kOutF16: return choose_linear<kOutF16, DUAL>(call);
