@@ -91,6 +91,7 @@ SIGNATURES = {
     "fl_mx_linear_swiglu": (C.c_int, [_vp, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _i32, _i32, _vp,
                                       _vp]),
     "fl_mx_status": (C.c_int, [C.POINTER(_i32), _i32, _vp]),
+    "fl_mx_give_up_at": (C.c_int, [_i32]),
 }
 
 # kernels launched by one call of an entry point (entry points that launch nothing are absent)

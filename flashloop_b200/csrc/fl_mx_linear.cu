@@ -12,7 +12,10 @@
 // which add their accumulators through distributed shared memory in rank order.
 //
 // Every wait on a copy or another CTA's sums is bounded: one that runs out raises a status word and the kernel runs to its
-// end.
+// end.  The warp that issues the matrix instructions gives up first: the warps that copy wait several times as long
+// for a stage that it frees, so that when one of them stops it has stopped long ago, and all stop at the same step, the ring's
+// length after its last.  A CTA (or pair) ends only when every copy under way has landed and every matrix
+// instruction is done.
 //
 // may_start_next() comes after a CTA has its tensor memory, so that a kernel let in early never holds columns
 // that this one still needs.  The other way round, a kernel that waits for the one before it holds few columns (few
@@ -32,6 +35,7 @@ namespace {
 constexpr int kLinThreads = 192;
 constexpr int kWaitTries = 1 << 15;  // of one wait, and for every step of K that it may have to sit through:
 constexpr int kWaitTriesPerStep = 256;
+constexpr int kCopierPatience = 4;  // times the tries of the waits between two stages that are freed
 constexpr int kTileW = 128 * 128;  // bytes of a staged weight tile
 constexpr int kMaxStages = 12;
 constexpr int kMaxSplits = 8;
@@ -66,11 +70,16 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   }
   return done != 0;
 }
+// The tries of a wait that may sit through this many steps of K.
+__device__ __forceinline__ int64_t tries_for(int steps) { return kWaitTries + int64_t(steps) * kWaitTriesPerStep; }
+__device__ __forceinline__ void report_timeout() { atomicExch(&g_mx_status, 1); }
+// Called by whole warps, whose lanes all get the same answer: what follows is uniform also where the tries ran out.
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int steps = 0) {
-  for (int64_t i = kWaitTries + int64_t(steps) * kWaitTriesPerStep; i > 0; --i)
-    if (mbar_try<CLUSTER>(bar, parity)) return true;
-  atomicExch(&g_mx_status, 1);
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int64_t tries = kWaitTries) {
+  bool done = false;
+  for (int64_t i = tries; i > 0 && !done; --i) done = mbar_try<CLUSTER>(bar, parity);
+  if (__any_sync(0xffffffffu, done)) return true;
+  report_timeout();
   return false;
 }
 // Position in a ring of stages and the parity of its current round.
@@ -81,6 +90,13 @@ struct Ring {
     if (++stage == stages) {
       stage = 0;
       parity ^= 1;
+    }
+  }
+  // Waits for the last copies into every stage of a ring that stands here, the first round of which is over if `again`.
+  __device__ __forceinline__ void drain(uint32_t full, int stages, bool again) const {
+    for (int s = 0; s < stages; ++s) {
+      const bool this_round = s < stage;
+      if (this_round || again) mbar_wait(full + 8 * s, this_round ? parity : parity ^ 1);
     }
   }
 };
@@ -252,6 +268,7 @@ struct LinearParams {
   uint32_t w_bytes, x_bytes;  // that the copies of one step's tiles report: a spread e2m1 tile counts as packed
   uint32_t idesc;
   uint32_t tmem_cols;
+  int give_up;  // step of a CTA's share whose copies are taken not to come (tests; never in its share otherwise)
 };
 
 // Shared memory of the kernel for few rows.
@@ -343,10 +360,12 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     // warp 0: weight tiles; 2: rows of x; 3: scales of x; 4: scales of the weights
     const uint8_t* x_scales = p.x_scales + int64_t(row0 / kMxTileRows) * p.steps * kMxTileBytes;
     const int64_t w_scales_at = int64_t(w_tile) * p.steps * kMxTileBytes;
+    const int end = min(last, first + p.give_up + p.stages);
     Ring ring_at;
-    for (int k = first; k < last; ++k, ring_at.advance(p.stages)) {
+    int k = first;
+    for (; k < end; ++k, ring_at.advance(p.stages)) {
       const int s = ring_at.stage;
-      if (k - first >= p.stages && !mbar_wait(empty + 8 * s, ring_at.parity ^ 1)) break;
+      if (k - first >= p.stages && !mbar_wait(empty + 8 * s, ring_at.parity ^ 1, kCopierPatience * kWaitTries)) break;
       const uint32_t at = ring + s * kStageBytes, bar = full + 8 * s;
       if (elect_one()) {
         if (warp == 0) {
@@ -368,17 +387,17 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       }
       __syncwarp();
     }
+    if (warp == 0) ring_at.drain(full, p.stages, k - first >= p.stages);  // a stage is full when all four have copied
   } else if (warp == 1) {
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const uint32_t tmem_scales = tmem + NT * kWeights;
     // scales of x: NT rows of a 128-row tile start at its column (row0 % 128) / 32, an even one
     const uint32_t x_col = 4 * kWeights + uint32_t(row0 % kMxTileRows) / 32;
+    const int end = min(last, first + p.give_up);
     Ring ring_at;
-    bool ok = true;
-    for (int k = first; k < last; ++k, ring_at.advance(p.stages)) {
+    for (int k = first; k < end; ++k, ring_at.advance(p.stages)) {
       const int s = ring_at.stage;
-      ok = mbar_wait(full + 8 * s, ring_at.parity);
-      if (!ok) break;
+      if (!mbar_wait(full + 8 * s, ring_at.parity)) break;
       const uint32_t at = ring + s * kStageBytes, scales = at + kScalesAt;
       const uint32_t sf = tmem_scales + s * Shape::kScaleCols;
       const uint64_t x_desc = tile_desc(at + kWeights * kTileW);
@@ -397,18 +416,17 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       }
       __syncwarp();
     }
+    if (end < last) report_timeout();
     if (elect_one()) commit_to(done);
     __syncwarp();
-    // after a wait that ran out: copies may still be landing
-    if (!ok)
-      for (int s = 0; s < p.stages; ++s) mbar_wait(full + 8 * s, ring_at.parity);
+    mbar_wait(done, 0, tries_for(p.steps));  // every product is done before tensor memory is given back
   }
   __syncwarp();
 
   const int n = w_tile * 128 + (warp & 3) * 32 + lane;
   if (warp >= 2) {
     const uint32_t acc = __shfl_sync(0xffffffffu, *tmem_slot, 0) + (uint32_t(warp & 3) * 32 << 16);
-    mbar_wait(done, 0, p.steps);
+    mbar_wait(done, 0, tries_for(p.steps));
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all of the cluster run
     const int feature = (warp & 3) * 32 + lane;
@@ -446,7 +464,7 @@ mx_linear_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     if (splits > 1 && my_groups > 0) {
       // The other CTAs always send, also after a wait of theirs has run out: wait as long as they may take.
-      for (int i = 0; i < 16 && !mbar_wait<true>(received, 0, p.steps); ++i) {
+      for (int i = 0; i < 16 && !mbar_wait<true>(received, 0, tries_for(p.steps)); ++i) {
       }
       for (int g = 0; g < my_groups; ++g) {
         const float4* src = exchange + g * 128 + feature;
@@ -537,6 +555,7 @@ struct PairParams {
   int64_t units;     // tiles times weights
   uint32_t stage_bytes;  // that the copies of one stage report, both CTAs
   uint32_t idesc;
+  int give_up;  // use of a stage by a pair whose copies are taken not to come (tests)
 };
 
 __device__ __forceinline__ void copy_tile_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -622,15 +641,19 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
     const uint32_t leader_full = in_cta(full, 0);
     Ring ring_at;
     bool ok = true, again = false;  // again: the ring has been filled once
+    int64_t left = int64_t(p.give_up) + kStages;  // uses of stages
     for (int64_t unit = pair * kWeights; ok && unit < p.units;
          unit += (DUAL && (unit & 1) == 0) ? 1 : pairs * kWeights - (DUAL ? 1 : 0)) {
       const int64_t tile = unit / kWeights;
       const int which = int(unit % kWeights);
       const int w_tile = int(tile % p.pair_tiles) * 2 + int(rank);
       const int row0 = int(tile / p.pair_tiles) * kPairRows;
-      for (int k = 0; k < p.steps; k += kSteps) {
+      const int end = int(min(int64_t(p.steps), left * kSteps));
+      left -= (p.steps + kSteps - 1) / kSteps;
+      ok = end == p.steps;
+      for (int k = 0; k < end; k += kSteps) {
         const int s = ring_at.stage;
-        if (again && !mbar_wait(empty + 8 * s, ring_at.parity ^ 1)) {
+        if (again && !mbar_wait(empty + 8 * s, ring_at.parity ^ 1, kCopierPatience * tries_for(p.steps))) {
           ok = false;
           break;
         }
@@ -657,23 +680,23 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
       }
     }
     // leave only when every copy of the pair has landed: the stages of this round, then those of the last
-    if (rank == 0) {
-      for (int s = 0; s < kStages; ++s) {
-        const bool this_round = s < ring_at.stage;
-        if (this_round || again) mbar_wait(full + 8 * s, this_round ? ring_at.parity : ring_at.parity ^ 1);
-      }
-    }
+    if (rank == 0) ring_at.drain(full, kStages, again);
   } else if (warp == 1 && rank == 0) {
     Ring ring_at, acc_at;
     bool ok = true, again = false;
+    int64_t left = p.give_up;
     for (int64_t unit = pair * kWeights; ok && unit < p.units;
          unit += (DUAL && (unit & 1) == 0) ? 1 : pairs * kWeights - (DUAL ? 1 : 0)) {
       const int buffer = acc_at.stage;
       const int row0 = int(unit / kWeights / p.pair_tiles) * kPairRows;
-      if (again && !mbar_wait<true>(acc_empty + 8 * buffer, acc_at.parity ^ 1, p.steps)) break;
+      if (again && !mbar_wait<true>(acc_empty + 8 * buffer, acc_at.parity ^ 1, tries_for(p.steps))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t acc = tmem + buffer * kPairRows;
-      for (int k = 0; k < p.steps; k += kSteps, ring_at.advance(kStages)) {
+      const int end = int(min(int64_t(p.steps), left * kSteps));
+      left -= (p.steps + kSteps - 1) / kSteps;
+      ok = end == p.steps;
+      if (!ok) report_timeout();
+      for (int k = 0; k < end; k += kSteps, ring_at.advance(kStages)) {
         const int s = ring_at.stage;
         if (!mbar_wait(full + 8 * s, ring_at.parity)) {
           ok = false;
@@ -707,7 +730,7 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
     // every product is done before tensor memory is given back
     if (elect_one()) commit_here(drained);
     __syncwarp();
-    mbar_wait(drained, 0, p.steps);
+    mbar_wait(drained, 0, tries_for(p.steps));
   } else if (warp >= 2) {
     const uint32_t quarter = uint32_t(warp & 3) * 32, part = uint32_t(warp - 2) / 4;
     constexpr int kCols = kPairRows / (kPairEpilogue<DUAL> / 4);  // this warp's columns of a tile
@@ -723,7 +746,7 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
       float gate[DUAL ? kCols : 1];
       if constexpr (DUAL) {
         const int buffer = acc_at.stage;
-        if (!mbar_wait(acc_full + 8 * buffer, acc_at.parity, 2 * p.steps)) break;
+        if (!mbar_wait(acc_full + 8 * buffer, acc_at.parity, tries_for(2 * p.steps))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
         for (int c = 0; c < kCols; c += 16) {
@@ -739,7 +762,7 @@ mx_linear_pair_kernel(const __grid_constant__ PairMaps maps, const PairParams p)
         acc_at.advance(2);
       }
       const int buffer = acc_at.stage;
-      if (!mbar_wait(acc_full + 8 * buffer, acc_at.parity, 2 * p.steps)) break;
+      if (!mbar_wait(acc_full + 8 * buffer, acc_at.parity, tries_for(2 * p.steps))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
       for (int c = 0; c < kCols; c += 16) {
@@ -836,6 +859,11 @@ struct LinearCall {
   int device;
 };
 
+// Step at which the kernels launched by this thread give up: none, but in tests.  More than any share has, and
+// 32 bits hold it with a share's first step and a ring's stages added.
+constexpr int kNever = 1 << 30;
+thread_local int t_give_up = kNever;
+
 template <int KIND, int NT, bool DUAL>
 int launch_linear(const LinearCall& call, int splits, int smem_limit) {
   using Shape = FewRows<NT, DUAL>;
@@ -863,6 +891,7 @@ int launch_linear(const LinearCall& call, int splits, int smem_limit) {
   // for columns in the same way) from sharing it.
   const int smem = std::max({1024 + kTailBytes + p.stages * Shape::kStageBytes + exchange,
                              int(p.tmem_cols) * (kSmemPerSm / 512) - 1024, kSmemHalf});
+  p.give_up = t_give_up;
   // instruction descriptor: element types (e4m3 0, e2m1 5), e8m0 scales, N, M = 128
   p.idesc = uint32_t(call.w[0].format == FL_MX_FP8 ? 0 : 5) << 7 | uint32_t(call.x.format == FL_MX_FP8 ? 0 : 5) << 10 |
             uint32_t(NT / 8) << 17 | 1u << 23 | uint32_t(128 / 16) << 24;
@@ -915,6 +944,7 @@ int launch_pairs(const LinearCall& call, int sms) {
   p.pair_tiles = (call.features + 255) / 256;
   const int64_t tiles = (call.rows + kPairRows - 1) / kPairRows * p.pair_tiles;
   p.units = tiles * (DUAL ? 2 : 1);
+  p.give_up = t_give_up;
   const bool w_spread = !PACKED && call.w[0].format == FL_MX_FP4, x_spread = !PACKED && call.x.format == FL_MX_FP4;
   p.stage_bytes = 2 * uint32_t((kTileW >> int(w_spread)) + (kPairXBytes >> int(x_spread)) + Shape::kScaleTiles * kMxTileBytes);
   // element types as in launch_linear, or e2m1 of kind::mxf4 (1)
@@ -1103,6 +1133,11 @@ extern "C" int fl_mx_linear_swiglu(const void* x_codes, const void* x_scales, in
   if (int rc = check_operand(who, "up", call.w[1])) return rc;
   FL_REQUIRE(out && aligned16(out) && aligned16(out_scales), "%s: outputs must be given, 16-byte aligned", who);
   return run_linear<true>(call);
+}
+
+extern "C" int fl_mx_give_up_at(int32_t step) {
+  t_give_up = step < 0 ? kNever : std::min(step, kNever);
+  return FL_OK;
 }
 
 extern "C" int fl_mx_status(int32_t* status, int32_t reset, fl_cuda_stream stream) {

@@ -517,6 +517,12 @@ int fl_mx_linear_swiglu(const void* x_codes, const void* x_scales, int32_t x_for
  * in the reference. */
 int fl_mx_status(int32_t* status, int32_t reset, fl_cuda_stream stream);
 
+/* A test's way of making waits run out: the projections that the calling host thread launches (or captures)
+ * from now on give up at the given step of K (of a CTA's share of them; with many rows, of the stages that a
+ * pair of CTAs uses one after the other), as if its copies did not come.  Negative: none does, as at the start.
+ * No counterpart in the reference. */
+int fl_mx_give_up_at(int32_t step);
+
 #ifdef __cplusplus
 }
 #endif
