@@ -11,7 +11,7 @@ from .cache import CrossLoopKVCache, CrossLoopKVLayer, CrossLoopKVLayerBuilder
 from .config import FlashLoopConfig
 from .engine import DecodeOutput, DecodeReceipt, EngineState, FlashLoopEngine, PrefillOutput
 from .kivi_backend import KiviPacked4Bit, pack_kivi_k_per_channel, pack_kivi_v_per_token
-from .mx import MXTensor, mx_linear, mx_linear_swiglu, mx_quantize, mx_rmsnorm
+from .mx import MXTensor, mx_linear, mx_linear_swiglu, mx_quantize, mx_rmsnorm, mx_status
 from .packing import Packed4Bit, pack_k_per_channel, pack_v_per_token
 from .selection import DecodeSelection, select_decode_keys, select_prefill_tokens
 
@@ -33,6 +33,7 @@ __all__ = [
     "mx_linear_swiglu",
     "mx_quantize",
     "mx_rmsnorm",
+    "mx_status",
     "pack_k_per_channel",
     "pack_kivi_k_per_channel",
     "pack_kivi_v_per_token",

@@ -24,7 +24,7 @@ from .cache import CrossLoopKVCache, CrossLoopKVLayer, CrossLoopKVLayerBuilder
 from .compaction import RetainedTokens, hidden_delta_score, retain_tokens
 from .config import FlashLoopConfig, validate_ouro_model
 from .selection import decode_budget
-from .mx import mx_linear, mx_linear_swiglu, mx_rmsnorm
+from .mx import mx_linear, mx_linear_swiglu, mx_rmsnorm, mx_status
 from .prefill import PrefillReceipt, apply_rope, dense_prefill_loop, norm_eps, sparse_prefill_loop
 from . import step_ops
 from .tensor_parallel import PartialSum, PeerAllReduce
@@ -146,6 +146,20 @@ class FlashLoopEngine:
         self._graph_warm = False
         self._decode_limit = 0
 
+    def _require_valid_products(self, device: torch.device, *, wait: bool) -> None:
+        """Raise, and drop the state, if a wait inside a microscaled projection has run out on ``device``.
+        Without ``wait`` only where nothing is under way on the stream, so that it costs no overlap."""
+
+        if self.projection_format is None:
+            return
+        if not wait and (torch.cuda.is_current_stream_capturing() or not torch.cuda.current_stream(device).query()):
+            return
+        if mx_status(device):
+            mx_status(device, reset=True)
+            self.reset()
+            raise RuntimeError("a bounded wait inside a microscaled projection ran out: what the engine returned "
+                               "since its last call that waited for the GPU is not valid, and its state is dropped")
+
     # ------------------------------------------------------------------ prefill
 
     def _retain(self, loop: int, scores: torch.Tensor, fraction: float,
@@ -208,7 +222,8 @@ class FlashLoopEngine:
 
         physical = CrossLoopKVCache(num_layers=len(self.layers))
         loops = (loop1, loop2, loop3, loop4)
-        rows3, rows4 = int(keep3.count[0]), int(keep4.count[0])
+        rows3, rows4 = int(keep3.count[0]), int(keep4.count[0])  # waits for all four loops
+        self._require_valid_products(input_ids.device, wait=True)
         for index, builder in enumerate(builders):
             physical.set_layer(index, builder.finalize(
                 loop3_positions=keep3.positions[:, :rows3], loop3_keys=loop3.updates[index][0],
@@ -516,7 +531,9 @@ class FlashLoopEngine:
 
     @torch.inference_mode()
     def decode(self, token_ids: torch.Tensor) -> DecodeOutput:
-        """engine.py:373-570 for one token per sequence, token_ids [B, 1]."""
+        """engine.py:373-570 for one token per sequence, token_ids [B, 1].  Returns without waiting for the GPU: with
+        microscaled projections a wait of theirs that ran out in this step is reported by a later call (or by
+        ``mx_status``, once the logits are there)."""
 
         state = self.state
         layers = state.cache.layers
@@ -525,6 +542,7 @@ class FlashLoopEngine:
             raise ValueError("decode requires exactly one token per sequence")
         if state.next_position >= self._decode_limit:
             raise RuntimeError("the preallocated cache is full; raise max_new_tokens")
+        self._require_valid_products(token_ids.device, wait=False)
         if self.use_cuda_graph:
             logits = self._graph_decode(token_ids)
         else:
@@ -575,4 +593,5 @@ class FlashLoopEngine:
                 break
             if step + 1 < int(max_new_tokens):
                 logits = self.decode(next_token).logits
+        self._require_valid_products(generated.device, wait=True)
         return generated
