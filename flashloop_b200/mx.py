@@ -16,7 +16,13 @@ import torch
 
 from . import _native
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone: a Stream object costs 2 us
+
+def _stream_handle(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the handle alone where this PyTorch has that call: a Stream object costs 2 us
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream_handle)
 
 FORMATS = {"mxfp8": 0, "mxfp4": 1}
 MAX_NORM_WIDTH = 8192

@@ -55,3 +55,23 @@ def test_threads_at_once():
         with ThreadPoolExecutor(4) as pool:
             assert [f.result() for f in [pool.submit(work, i, own_stream) for i in range(4)]] == [30] * 4
     assert mx_status() == 0
+
+
+def test_streams_without_the_raw_handle(monkeypatch):
+    """What a PyTorch without that call uses names the same stream."""
+
+    from flashloop_b200 import mx
+
+    x, out = torch.zeros(4, 256, device="cuda"), []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for handle in (mx._raw_stream, mx._stream_handle):
+        monkeypatch.setattr(mx, "_raw_stream", handle)
+        with torch.cuda.stream(side):
+            assert handle(side.device_index) == side.cuda_stream
+            torch.cuda._sleep(2_000_000)  # about a millisecond
+            out.append(fl.mx_quantize(x.fill_(3.0)).dequantize())
+            x.zero_()
+        assert handle(0) == torch.cuda.current_stream().cuda_stream
+    torch.cuda.synchronize()
+    assert all(bool((o == 3).all()) for o in out)
