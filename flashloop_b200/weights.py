@@ -11,7 +11,7 @@ import torch
 from torch import nn
 from torch.nn import functional as F
 
-from .mx import MXTensor, mx_linear, mx_linear_swiglu, mx_quantize
+from .mx import MXTensor, _format_code, mx_linear, mx_linear_swiglu, mx_quantize
 
 
 @torch.no_grad()
@@ -44,32 +44,42 @@ def repack_projection_weights(layers: Sequence[nn.Module]) -> None:
 @torch.no_grad()
 def quantize_projection_weights(layers: Sequence[nn.Module], format: str) -> None:
     """Replace the repacked projection weights of every layer (Q/K/V, ``o_proj``, gate, up,
-    ``down_proj``) by their microscaled form and release the bfloat16 tensors.  No counterpart in the
-    reference, whose projections stay bfloat16 (flashloop/weights.py:20-117)."""
+    ``down_proj``) by their microscaled form and release the bfloat16 tensors: all of them once every
+    microscaled one is there, or none.  No counterpart in the reference, whose projections stay
+    bfloat16 (flashloop/weights.py:20-117)."""
 
-    for layer in layers:
+    _format_code(format)
+    todo = []
+    for layer in layers:  # what is refused is refused before anything changes
         attention, mlp = layer.self_attn, layer.mlp
         done = getattr(attention, "_flashloop_mx_qkv", None)
         if done is not None:
             if done.format != format:
                 raise RuntimeError(f"the projections are already held in {done.format}")
             continue
-        if not hasattr(attention, "_flashloop_qkv_weight") or not hasattr(mlp, "_flashloop_gate_up_weight"):
+        if (getattr(attention, "_flashloop_qkv_weight", None) is None
+                or getattr(mlp, "_flashloop_gate_up_weight", None) is None):
             raise ValueError("microscaled projections need fused projection weights (repack_projection_weights)")
         for name, module in (("o_proj", attention.o_proj), ("down_proj", mlp.down_proj)):
             if module.bias is not None:
                 raise ValueError(f"microscaled projections require biasless {name}")
-        qkv = mx_quantize(attention._flashloop_qkv_weight, format)
-        value_row = sum(attention._flashloop_qkv_splits[:2])
-        if value_row % 128:
+            if module.weight is None:
+                raise ValueError(f"{name} has already released its weight")
+        if sum(attention._flashloop_qkv_splits[:2]) % 128:
             raise ValueError("microscaled projections need heads of 128 channels")
+        todo.append((attention, mlp))
+    made = []
+    for attention, mlp in todo:  # which may run out of memory
         gate, up = mlp._flashloop_gate_up_weight.split(mlp._flashloop_gate_up_splits, dim=0)
+        made.append([mx_quantize(w, format) for w in (attention._flashloop_qkv_weight, attention.o_proj.weight, gate, up,
+                                                      mlp.down_proj.weight)])
+    for (attention, mlp), (qkv, output, gate, up, down) in zip(todo, made):
+        value_row = sum(attention._flashloop_qkv_splits[:2])
         attention._flashloop_mx_qkv = qkv
         attention._flashloop_mx_value = MXTensor(qkv.codes[value_row:], qkv.scales[value_row // 128:],
                                                  (attention._flashloop_qkv_splits[2], qkv.cols), format)
-        attention._flashloop_mx_output = mx_quantize(attention.o_proj.weight, format)
-        mlp._flashloop_mx_gate, mlp._flashloop_mx_up = mx_quantize(gate, format), mx_quantize(up, format)
-        mlp._flashloop_mx_down = mx_quantize(mlp.down_proj.weight, format)
+        attention._flashloop_mx_output = output
+        mlp._flashloop_mx_gate, mlp._flashloop_mx_up, mlp._flashloop_mx_down = gate, up, down
         attention._flashloop_qkv_weight = mlp._flashloop_gate_up_weight = None
         attention.o_proj.weight = mlp.down_proj.weight = None
 
