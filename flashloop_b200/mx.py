@@ -4,7 +4,7 @@
 Thirty-two consecutive elements of a row share a power-of-two scale; the elements are e4m3
 (``"mxfp8"``) or e2m1 (``"mxfp4"``).  The reference's projections are bfloat16
 (flashloop/weights.py:74-117); these are what ``FlashLoopEngine(projection_format=...)`` runs
-instead.  Inference only: no gradient is recorded, and inputs that require one are refused.
+instead.  Inference only: no gradient is recorded, and inputs that require one, or carry a tangent, are refused.
 """
 
 from __future__ import annotations
@@ -13,6 +13,7 @@ import ctypes as C
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 
@@ -213,6 +214,14 @@ def _values(x: torch.Tensor, *others: torch.Tensor | None) -> None:
                 raise RuntimeError(_NO_GRADIENT)
     if grad and x.requires_grad:
         raise RuntimeError(_NO_GRADIENT)
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # inside a dual level: asking every tensor takes 0.4 us each
+        _refuse_duals(x, *others)
+
+
+def _refuse_duals(*tensors: torch.Tensor | None) -> None:
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("microscaled operators record no gradient: a dual tensor would lose its tangent")
 
 
 _NO_GRADIENT = "microscaled operators record no gradient: call them under torch.no_grad()"
