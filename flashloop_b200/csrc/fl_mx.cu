@@ -184,6 +184,7 @@ extern "C" int fl_mx_quantize(const void* x, int32_t x_dtype, int64_t rows, int3
   FL_REQUIRE(rows >= 0 && cols > 0 && (row_stride >= cols || rows <= 1), "%s: bad sizes", who);
   if (rows == 0) return FL_OK;
   FL_REQUIRE(x && codes && scales, "%s: null argument", who);
+  FL_REQUIRE(aligned_to(x, x_dtype), "%s: x must be aligned to its elements", who);
   FL_REQUIRE(aligned16(codes) && aligned16(scales), "%s: codes and scales must be 16-byte aligned", who);
   return by_type_and_format(x_dtype, format, QuantizeCall{x, rows, cols, row_stride, codes, scales,
                                                           static_cast<cudaStream_t>(stream)});

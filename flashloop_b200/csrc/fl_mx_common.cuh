@@ -391,6 +391,10 @@ int by_type_and_format(int dtype, int format, F&& f) {
       return fp8 ? f.template run<float, FL_MX_FP8>() : f.template run<float, FL_MX_FP4>();
   }
 }
+// Whether an address is one of an element of this type (null is).
+inline bool aligned_to(const void* p, int dtype) {
+  return (reinterpret_cast<uintptr_t>(p) & (dtype == FL_DTYPE_F32 ? 3u : 1u)) == 0;
+}
 inline bool dtype_ok(int dtype) { return dtype == FL_DTYPE_BF16 || dtype == FL_DTYPE_F16 || dtype == FL_DTYPE_F32; }
 
 #endif  // __CUDACC__

@@ -296,6 +296,8 @@ extern "C" int fl_rmsnorm_mx(const void* x, const void* addend, const void* resi
   FL_REQUIRE(residual == nullptr || weight2 != nullptr, "%s: a residual needs weight2", who);
   FL_REQUIRE(sum_out == nullptr || addend != nullptr, "%s: sum_out needs an addend", who);
   FL_REQUIRE(x && weight && codes && scales, "%s: null argument", who);
+  for (const void* p : {x, addend, residual, weight, weight2, static_cast<const void*>(sum_out), static_cast<const void*>(hidden)})
+    FL_REQUIRE(aligned_to(p, dtype), "%s: tensors must be aligned to their elements", who);
   FL_REQUIRE(aligned16(codes) && aligned16(scales), "%s: codes and scales must be 16-byte aligned", who);
   return by_type_and_format(dtype, format,
                             NormCall{{x, addend, residual, weight, weight2, eps, eps2, rows, width, sum_out, hidden,

@@ -477,7 +477,8 @@ int64_t fl_mx_codes_bytes(int64_t rows, int32_t cols, int32_t format);
 /* No counterpart in the reference. */
 int64_t fl_mx_scales_bytes(int64_t rows, int32_t cols);
 
-/* x [rows][cols] of x_dtype, rows row_stride elements apart -> codes and scales (16-byte aligned).
+/* x [rows][cols] of x_dtype (aligned to its elements), rows row_stride elements apart -> codes and scales
+ * (16-byte aligned).
  * No counterpart in the reference. */
 int fl_mx_quantize(const void* x, int32_t x_dtype, int64_t rows, int32_t cols, int64_t row_stride,
                    int32_t format, void* codes, void* scales, fl_cuda_stream stream);
@@ -490,8 +491,8 @@ int fl_mx_dequantize(const void* codes, const void* scales, int32_t format, int6
  * reference has no such output).  s = x, or with addend s = round(addend + x), stored to sum_out if
  * given; n = weight * s * rsqrt(mean(s^2) + eps).  Without weight2 the codes are those of n; with it
  * hidden = round([residual +] n) and the codes are those of weight2 * hidden * rsqrt(mean(hidden^2) +
- * eps2).  x, addend, residual, weight, weight2, sum_out, hidden are of one dtype, rows contiguous, 1 to
- * 8192 wide; between the stored tensors everything is float32 (unlike fl_rmsnorm, which rounds where
+ * eps2).  x, addend, residual, weight, weight2, sum_out, hidden are of one dtype, aligned to its elements, rows
+ * contiguous, 1 to 8192 wide; between the stored tensors everything is float32 (unlike fl_rmsnorm, which rounds where
  * bfloat16 tensor ops would). */
 int fl_rmsnorm_mx(const void* x, const void* addend, const void* residual, const void* weight, float eps,
                   const void* weight2, float eps2, int32_t dtype, int64_t rows, int32_t width, int32_t format,
