@@ -87,6 +87,12 @@ def parse_args():
                          "peer memory, replayed from a CUDA graph; nccl = NCCL all-reduces, launched eagerly")
     ap.add_argument("--no-tp-probe", action="store_true", help="N>1 replica runs: skip the tensor-parallel measurement")
     ap.add_argument("--no-graph", action="store_true", help="launch every step eagerly instead of replaying a CUDA graph")
+    ap.add_argument("--projection-format", default=None, choices=["mxfp4", "mxfp8"],
+                    help="e2e workload: projections on microscaled operands instead of bfloat16 ones (a different "
+                         "precision: not the headline number)")
+    ap.add_argument("--time-prefill", action="store_true",
+                    help="e2e workload on one GPU: prefill once more after everything else, when nothing is set up for "
+                         "the first time (details.prefill_warm_seconds)")
     ap.add_argument("--no-probes", action="store_true",
                     help="skip the configs[1]-shaped reader probes behind roofline_dense / roofline_sparse")
     ap.add_argument("--update-traffic", metavar="CSV", nargs="+", default=None,
@@ -105,6 +111,8 @@ def parse_args():
         args.context = {"hotpath": CONTEXT, "ragged": 32768, "e2e": 2048, "kernels": CONTEXT}[args.workload]
     if args.layers is None:
         args.layers = 1 if args.workload == "ragged" else LAYERS
+    if args.projection_format and (args.workload != "e2e" or args.tp):
+        ap.error("--projection-format goes with the e2e workload, without --tp")
     return args
 
 
@@ -137,7 +145,8 @@ def bench_config(args) -> dict:
     else:
         l2 = "inputs larger than L2: each step streams the packed cache of every layer"
         parallelism = f"batch-sharded x{world}, no data-path collective"
-    return {"workload": workload_name(args), "global_batch": args.batch if tp else args.batch * world, "l2": l2,
+    extra = {"projections": args.projection_format} if getattr(args, "projection_format", None) else {}
+    return {**extra, "workload": workload_name(args), "global_batch": args.batch if tp else args.batch * world, "l2": l2,
             "parallelism": parallelism,
             "launch": ("eager" if args.no_graph or (tp and getattr(args, "tp_allreduce", "peer") == "nccl")
                        else "one CUDA graph replay per step")}
@@ -1043,7 +1052,8 @@ def run_e2e(args) -> None:
     graph_ok = not args.no_graph and not (tp and args.tp_allreduce == "nccl")
     engine = FlashLoopEngine(model, config=FlashLoopConfig(kv_bits=args.bits), validate_model=False,
                              max_new_tokens=budget, use_cuda_graph=graph_ok,
-                             tp_group=dist.group.WORLD if tp else None, tp_allreduce=args.tp_allreduce)
+                             tp_group=dist.group.WORLD if tp else None, tp_allreduce=args.tp_allreduce,
+                             projection_format=args.projection_format)
     gen = torch.Generator().manual_seed(100 + (0 if tp else rank))
     prompts = torch.randint(0, cfg.vocab_size, (B, T), generator=gen).to(device)
     torch.cuda.synchronize()
@@ -1054,6 +1064,7 @@ def run_e2e(args) -> None:
     torch.cuda.synchronize()
     prefill_s = time.perf_counter() - t0
     prefill_peak = torch.cuda.max_memory_allocated(device) - before_prefill
+    held = torch.cuda.memory_allocated(device)
     state = {"token": logits.argmax(-1, keepdim=True)}
 
     def run_step():
@@ -1136,13 +1147,14 @@ def run_e2e(args) -> None:
     probes = {}
     if rank == 0 and not args.no_probes:
         probes = probe_configs1_readers(device, args.bits)
-        probes.update(probe_projection(model, B, device))
+        if not args.projection_format:
+            probes.update(probe_projection(model, B, device))
     if world > 1:
         dist.barrier()
 
     # ---- N>1 replica runs: the same model once more, sharded over the ranks (strong scaling)
     tensor_parallel = None
-    if world > 1 and not tp and not args.no_tp_probe:
+    if world > 1 and not tp and not args.no_tp_probe and not args.projection_format:
         # every rank takes the same branch at every step: a rank that fails tells the others before the
         # next collective, so nobody is left waiting in one
         def all_ok(ok: bool) -> bool:
@@ -1187,11 +1199,17 @@ def run_e2e(args) -> None:
         line = {
             "metric": METRIC, "value": value, "unit": "tok/s", "n_gpus": world, "steps": args.steps,
             "warmup": args.warmup, "ms_per_step": ms_total / args.steps, "higher_is_better": True,
-            "scaling": "strong" if tp else "weak", "vs_baseline": None, "dtype": "bf16", "data": "synthetic",
+            "scaling": "strong" if tp else "weak", "vs_baseline": None,
+            "dtype": f"bf16, projections {args.projection_format}" if args.projection_format else "bf16", "data": "synthetic",
             "config": bench_config(args),
             "details": {"prefill_seconds": prefill_s, "prefill_peak_bytes_above_model": prefill_peak,
+                        "bytes_held_after_prefill": held,
                         "cache_storage_bytes": engine.state.cache.storage_bytes, "context_at_end": quant + tail,
-                        "weight_bytes_streamed_per_step": 4 * weights},
+                        **({"projection_weight_bytes": sum(
+                            w.nbytes() for layer in model.model.layers for w in (
+                                layer.self_attn._flashloop_mx_qkv, layer.self_attn._flashloop_mx_output,
+                                layer.mlp._flashloop_mx_gate, layer.mlp._flashloop_mx_up, layer.mlp._flashloop_mx_down))}
+                           if args.projection_format else {"weight_bytes_streamed_per_step": 4 * weights})},
             "clocks": clocks,
             "e2e": {"value": e2e_value, "unit": "tok/s", "h2d_bytes_per_step": int(host_token.numel() * 8),
                     "d2h_bytes_per_step": int(host_token.numel() * 8), "steps": e2e_steps},
@@ -1208,6 +1226,13 @@ def run_e2e(args) -> None:
             "reader_status": status,
         }
         line.update(probes)
+        if args.time_prefill and world == 1:
+            engine.reset()
+            torch.cuda.synchronize()
+            t0 = time.perf_counter()
+            engine.prefill(prompts)
+            torch.cuda.synchronize()
+            line["details"]["prefill_warm_seconds"] = time.perf_counter() - t0
         if tensor_parallel is not None:
             line["tensor_parallel"] = tensor_parallel
         if tp:
