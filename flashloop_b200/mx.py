@@ -26,6 +26,7 @@ def _stream_handle(index: int) -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream_handle)
 
 FORMATS = {"mxfp8": 0, "mxfp4": 1}
+_CODE_TYPES = ("float8_e4m3fn", "float4_e2m1fn_x2")  # by format code, where this PyTorch has them
 MAX_NORM_WIDTH = 8192
 MAX_COLUMNS = 2**31 - 256  # of a row: the kernels index a row in 32 bits
 
@@ -98,17 +99,19 @@ class MXTensor:
     @classmethod
     def from_row_scales(cls, codes: torch.Tensor, scales: torch.Tensor, shape, format: str) -> "MXTensor":
         """From the plain layout of a checkpoint: ``codes`` [rows, cols] (mxfp8) or [rows, ceil(cols / 2)] (mxfp4, the
-        even element in the low nibble) and ``scales`` [rows, ceil(cols / 32)], uint8 or the float8 types of the
-        same bytes; padded and tiled once, by tensor operations on whatever device they are."""
+        even element in the low nibble) and ``scales`` [rows, ceil(cols / 32)], as uint8, int8 or the types of just
+        these bytes (float8_e4m3fn, float4_e2m1fn_x2, float8_e8m0fnu); padded and tiled once, by tensor operations
+        on whatever device they are."""
 
         shape = tuple(int(v) for v in shape)
         if not shape or min(shape) < 0 or not 0 < shape[-1] <= MAX_COLUMNS:
             raise ValueError(f"a microscaled tensor needs a last dimension of 1 to {MAX_COLUMNS}")
         rows, cols, code = math.prod(shape[:-1]), shape[-1], _format_code(format)
-        for t, want, name in ((codes, (rows, -(-cols // 2) if code else cols), "codes"),
-                              (scales, (rows, -(-cols // 32)), "scales")):
-            if t.element_size() != 1 or tuple(t.shape) != want:
-                raise ValueError(f"{name} of {shape} in {format} must be one byte each, {want}, got {tuple(t.shape)} {t.dtype}")
+        for t, want, name, own in ((codes, (rows, -(-cols // 2) if code else cols), "codes", _CODE_TYPES[code]),
+                                   (scales, (rows, -(-cols // 32)), "scales", "float8_e8m0fnu")):
+            if t.dtype not in (torch.uint8, torch.int8, getattr(torch, own, None)) or tuple(t.shape) != want:
+                raise ValueError(f"{name} of {shape} in {format} must be uint8, int8 or {own}, {want}, "
+                                 f"got {tuple(t.shape)} {t.dtype}")
         codes, scales = codes.view(torch.uint8), scales.view(torch.uint8)
         if code and cols % 2:
             codes = codes.clone()
