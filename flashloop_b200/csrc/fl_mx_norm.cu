@@ -69,7 +69,7 @@ __device__ __forceinline__ float inverse_root(float sum, int width, float eps) {
 // LANES threads share a row and hold it in registers, CHUNKS times sixteen elements per thread; as few as hold it, eight
 // (one scale word) at least.  CTAs take rows one after the other and ask for the next ones before they work on the
 // present ones: bound by memory with many rows (bfloat16, residual and second norm: 32768 x
-// 2048 79 us, 0.92 of the copy rate; 100000 x 192 38 us, 0.55; rows of 2047, which go through shared memory, 151 us), by
+// 2048 79 us, 0.92 of the copy rate; 100000 x 192 36 us, 0.6; rows of 2047, which go through shared memory, 145 us), by
 // latency with few (16 x 2048: 2.2 us).
 template <int LANES>
 constexpr int kNormThreads = LANES < 128 ? 128 : LANES;
