@@ -147,18 +147,19 @@ class FlashLoopEngine:
         self._decode_limit = 0
 
     def _require_valid_products(self, device: torch.device, *, wait: bool) -> None:
-        """Raise, and drop the state, if a wait inside a microscaled projection has run out on ``device``.
-        Without ``wait`` only where nothing is under way on the stream, so that it costs no overlap."""
+        """Raise, and drop the state, if a wait inside a microscaled projection has run out on ``device`` since the
+        status was last reset: it stays set, as other engines on the device have to see it too.  Without ``wait``
+        only where nothing is under way on the stream, so that it costs no overlap."""
 
         if self.projection_format is None:
             return
         if not wait and (torch.cuda.is_current_stream_capturing() or not torch.cuda.current_stream(device).query()):
             return
         if mx_status(device):
-            mx_status(device, reset=True)
             self.reset()
-            raise RuntimeError("a bounded wait inside a microscaled projection ran out: what the engine returned "
-                               "since its last call that waited for the GPU is not valid, and its state is dropped")
+            raise RuntimeError("a bounded wait inside a microscaled projection ran out: what engines on this device "
+                               "returned since their last call that waited for the GPU is not valid, and this one's "
+                               "state is dropped; mx_status(device, reset=True) clears the status")
 
     # ------------------------------------------------------------------ prefill
 

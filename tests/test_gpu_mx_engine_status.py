@@ -36,9 +36,11 @@ def test_prefill_raises_and_can_be_repeated(give_up_at):
     with pytest.raises(RuntimeError, match="ran out"):
         engine.prefill(prompts)
     give_up_at(-1)
-    assert mx_status() == 0
     with pytest.raises(RuntimeError, match="not initialized"):
         engine.decode(prompts[:, :1])
+    with pytest.raises(RuntimeError, match="ran out"):  # until somebody has taken note
+        engine.prefill(prompts)
+    assert mx_status(reset=True) == 1
     assert torch.equal(engine.prefill(prompts).logits, want)
 
 
@@ -58,7 +60,7 @@ def test_generate_raises(graph, give_up_at):
         engine.generate(prompts, max_new_tokens=5, eos_token_id=-1)
     give_up_at(-1)
     del engine.decode
-    assert mx_status() == 0
+    assert mx_status(reset=True) == 1
     assert engine.generate(prompts, max_new_tokens=5).shape[0] == 2
 
 
@@ -78,8 +80,22 @@ def test_decode_raises_in_the_step_after(graph, give_up_at):
         engine.decode(token)
     with pytest.raises(RuntimeError, match="not initialized"):
         engine.decode(token)
+    assert mx_status(reset=True) == 1
     engine.prefill(prompts)
     engine.decode(token)
+
+
+def test_every_engine_on_the_device_sees_it(give_up_at):
+    prompts, one, other = PROMPTS.cuda(), _engine(), _engine()
+    token = prompts[:, :1].contiguous()
+    for engine in (one, other):
+        engine.prefill(prompts)
+    give_up_at(0)
+    one.decode(token).logits.cpu()
+    give_up_at(-1)
+    for engine in (other, one):  # whoever looks first
+        with pytest.raises(RuntimeError, match="ran out"):
+            engine.decode(token)
 
 
 def test_bfloat16_projections_do_not_look_at_it(give_up_at):
